@@ -14,6 +14,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libcwen_cuda.so"
 
 CWEN_T_F32, CWEN_T_Q4_0, CWEN_T_Q8_0 = 0, 2, 8
+CWEN_T_F16, CWEN_T_BF16 = 1, 30  # element types of the attention operators, with CWEN_T_F32
 
 
 class Dims(C.Structure):
@@ -30,11 +31,23 @@ class SpecStats(C.Structure):
     _fields_ = [(n, C.c_longlong) for n in ("cycles", "drafted", "full", "shortw", "kept", "plain_steps")]
 
 
+class Rope(C.Structure):
+    _fields_ = [("n_rot", C.c_int), ("half", C.c_int), ("mscale", C.c_float), ("reserved", C.c_int),
+                ("turn", C.c_double * 128)]
+
+
+class Kv(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "n_layer", "n_pages", "page_size", "n_kv", "head_dim")] + [
+        ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
 class CwenError(RuntimeError):
     pass
 
 
 _lib = None
+
+_P, _I, _L = C.c_void_p, C.c_int, C.c_int64
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -58,6 +71,17 @@ _SIGS = {
     "cwen_cuda_gdn_verify": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
                                        C.c_void_p]),
+    "cwen_rope_init": (_I, [C.POINTER(Rope), _I, _I] + [C.c_double] * 5),
+    "cwen_cuda_rope": (_I, [C.POINTER(Rope), _I, _I, _I, _I, _P, _L, _L, _P, _I, _P, _L, _L, _P]),
+    "cwen_cuda_kv_append": (_I, [C.POINTER(Kv), _I, _P, _I, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _P,
+                                 C.POINTER(Rope), _P, _P]),
+    "cwen_cuda_kv_compact": (_I, [C.POINTER(Kv), _P, _I, _I, _P, _P, _P, _P]),
+    "cwen_cuda_attn_prompt": (_I, [_I, _I, _P, _I, _I, _I, _I, C.c_float, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L,
+                                   _L, _P]),
+    "cwen_cuda_attn_tree": (_I, [C.POINTER(Kv), _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, C.c_float, _P, _L, _L, _P, _L,
+                                 _L, _P, C.c_size_t, _P]),
+    "cwen_cuda_attn_tree_ws": (C.c_size_t, [C.POINTER(Kv), _I, _I, _I]),
+    "cwen_cuda_attn_status": (_I, [_P]),
     "cwen_cuda_model_config": (C.c_int, [C.POINTER(Dims)]),
     "cwen_cuda_upload": (C.c_int, [C.c_char_p, C.c_int, C.c_void_p, C.c_int, C.c_int]),
     "cwen_cuda_model_finalize": (C.c_int, []),

@@ -28,7 +28,7 @@ CFLAGS = ["-O2", "-std=gnu11", "-fPIC", "-Wall", "-Wextra", "-I" + str(PKG / "ho
 
 
 def _headers() -> list[Path]:
-    return list((PKG / "csrc").glob("*.cuh")) + list((PKG / "host").glob("*.h")) + [ROOT / "include" / "cwen_cuda.h"]
+    return list((PKG / "csrc").glob("*.cuh")) + list((PKG / "csrc").glob("*.h")) + list((PKG / "host").glob("*.h")) + [ROOT / "include" / "cwen_cuda.h"]
 
 
 def _stale(obj: Path, src: Path, deps: list[Path]) -> bool:

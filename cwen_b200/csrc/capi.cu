@@ -5,6 +5,7 @@
 
 #include "engine.cuh"
 #include "attn.cuh"
+#include "attnops.cuh"
 #include "gdn.cuh"
 #include "model.cuh"
 #include "qmv.cuh"
@@ -166,6 +167,8 @@ int cwen_cuda_init(int device, int ctx, int bmax) {
   CW_CHECK(rowops_configure());
   CW_CHECK(attn_configure());
   CW_CHECK(gdn_configure());
+  CW_CHECK(kvops_configure());
+  CW_CHECK(attnops_configure());
   E.device = device;
   E.ctx = ctx;
   E.bmax = bmax;
@@ -194,6 +197,8 @@ int cwen_cuda_init(int device, int ctx, int bmax) {
   CW_CHECK(cudaMalloc(&s.stat_next, (size_t)160 * QG_STAT_COLS * sizeof(float)));
   CW_CHECK(cudaMalloc(&E.aw, argmax_part_bytes(QG_MAXB)));
   CW_CHECK(cudaMemset(E.aw, 0, argmax_part_bytes(QG_MAXB)));
+  CW_CHECK(cudaMalloc(&E.op_err, sizeof(int)));
+  CW_CHECK(cudaMemset(E.op_err, 0, sizeof(int)));
   CW_CHECK(cudaMalloc(&E.aw_res, (2 + QG_MAXB) * sizeof(int)));
   E.live = true;
   return CWEN_OK;
@@ -223,6 +228,7 @@ void cwen_cuda_shutdown(void) {
   cudaFree(E.gs.stat_next);
   cudaFree(E.aw);
   cudaFree(E.aw_res);
+  cudaFree(E.op_err);
   if (E.staging) cudaFree(E.staging);
   if (E.io) cudaFree(E.io);
   cudaStreamDestroy(E.stream);

@@ -33,6 +33,7 @@ struct Engine {
   size_t staging_bytes = 0;
   void *aw = nullptr;    // argmax + walk scratch of cwen_cuda_accept_logits
   int *aw_res = nullptr; // its result row [2 + 16]
+  int *op_err = nullptr;  // flag of the attention operators (attnops.cuh), read by cwen_cuda_attn_status
   float *io = nullptr;  // device buffers for the host-buffer entry points
   size_t io_floats = 0;
   Prof prof;

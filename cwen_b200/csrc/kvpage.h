@@ -1,0 +1,39 @@
+// Page-table arithmetic of the paged cache, for the kernels and the host.
+//
+// A cache pool is [layer][page][slot in the page][kv head][head_dim]; a
+// sequence's table row holds the page ids of its slots in order.  Page ids
+// come from device memory that the host cannot check, so every lookup is
+// checked here and a bad one gives -1: nothing outside the pool is touched.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define CWP_FN __host__ __device__ __forceinline__
+#else
+#define CWP_FN static inline
+#endif
+
+// Pool row (page * page_size + slot in the page) of a sequence's `slot`, or
+// -1 when the slot lies outside the table row or its page id outside
+// [0, n_pages).  64 bits: a pool may hold more than 2^31 rows' elements.
+CWP_FN int64_t cwp_row(const int *table_row, int table_stride, int n_pages, int page_size, int64_t slot) {
+  if (slot < 0 || slot >= (int64_t)table_stride * page_size) return -1;
+  // in range, slot / page_size < table_stride: 32-bit arithmetic where it can be
+  const int64_t p = slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
+  const int page = table_row[p];
+  if (page < 0 || page >= n_pages) return -1;
+  return (int64_t)page * page_size + (slot - p * page_size);
+}
+
+// Slot of the i-th set bit (from the lowest) of a 64-bit keep mask; -1 past the last.
+CWP_FN int cwp_nth_bit(uint64_t m, int i) {
+  for (; m; m &= m - 1)
+    if (i-- == 0) {
+#ifdef __CUDA_ARCH__
+      return __ffsll((long long)m) - 1;
+#else
+      return __builtin_ctzll(m);
+#endif
+    }
+  return -1;
+}

@@ -35,6 +35,8 @@ enum {
 
 /* ggml tensor types accepted by the upload calls (GGUF numbering). */
 enum { CWEN_T_F32 = 0, CWEN_T_Q4_0 = 2, CWEN_T_Q8_0 = 8 };
+/* With CWEN_T_F32, the element types of the attention operators (GGUF numbering). */
+enum { CWEN_T_F16 = 1, CWEN_T_BF16 = 30 };
 
 /* Model geometry; the reference fixes it at compile time (run.c:83-91). */
 typedef struct {
@@ -212,6 +214,100 @@ int cwen_cuda_gdn_state(int layer, float *S_host, float *conv_host);
  * One kernel launch on `stream` (NULL: the engine's); synchronizes. */
 int cwen_cuda_accept_logits(const float *dlogits, int n, int ldl, int B, const int *blk, int E_drafts, int *res,
                             void *stream);
+
+/* ---- attention operators on caller device buffers ----
+ * Rotary positions, a paged K/V cache, attention over whole prompts and over
+ * drafted trees, for callers that keep several sequences: rope the queries,
+ * append the (roped) keys and the values to the pages, attend, compact the
+ * accepted path.  The engine's own decode path does not use them (it keeps one
+ * sequence's contiguous fp32 cache).  Common rules:
+ *  - rows are element (r, h, d) at p[r*row + h*head + d], strides in elements;
+ *    any stride and alignment is accepted (16-byte aligned rows are faster);
+ *  - buffers live on the engine's GPU; work is ordered on `stream` (NULL: the
+ *    engine's stream; the legacy default stream is cudaStreamLegacy); calls
+ *    do not synchronize or allocate and can be captured into graphs;
+ *  - types are CWEN_T_F32, CWEN_T_F16, CWEN_T_BF16; softmax statistics and sums
+ *    are fp32, each result is rounded once;
+ *  - device arrays (lengths, slots, page ids) cannot be checked on the host:
+ *    what is out of range is never dereferenced, its rows or slots are left
+ *    out, and cwen_cuda_attn_status reports it.
+ * Output buffers must not overlap inputs except where said. */
+
+/* Rotary positions: pair i < n_rot/2 of a head turns by 2 pi pos turn[i] and is
+ * scaled by mscale.  The pairs are dims (2i, 2i+1) (half = 0; run.c's rope) or
+ * (i, i + n_rot/2) (half = 1); dims from n_rot on pass unchanged.  A plain host
+ * struct without device state: copy it, or set turn[] for another scaling. */
+typedef struct {
+  int n_rot, half;
+  float mscale;
+  int reserved;
+  double turn[128];
+} cwen_rope;
+/* turn[i] = base^(-2i/n_rot) / 2 pi, scaled for long contexts: with beta_fast =
+ * beta_slow = 0 linearly (turn / factor; 1 = unscaled), else by parts (the
+ * YaRN paper, arXiv:2309.00071, section 3.2 and eq. 22): a pair that makes
+ * n = orig_ctx turn[i] turns over the trained context keeps the share
+ * g = clamp((n - beta_slow) / (beta_fast - beta_slow), 0, 1) of its turn,
+ * turn (g + (1 - g) / factor), and mscale = 0.1 ln(factor) + 1. */
+int cwen_rope_init(cwen_rope *r, int n_rot, int half, double base, double factor, double orig_ctx, double beta_fast,
+                   double beta_slow);
+/* y = rope(x) for n_rows rows of n_head heads of head_dim <= 512 dims, row r at
+ * position pos[r] (any int); inverse turns back (the gradient, and moving
+ * cached keys).  y may be x with the same strides. */
+int cwen_cuda_rope(const cwen_rope *r, int type, int n_rows, int n_head, int head_dim, const void *x, int64_t xrow,
+                   int64_t xhead, const int *pos, int inverse, void *y, int64_t yrow, int64_t yhead, void *stream);
+
+/* A paged cache: k and v are [n_layer][n_pages][page_size][n_kv][head_dim],
+ * 16-byte aligned, head_dim a multiple of 8.  Slot t of sequence s is in page
+ * table[s*table_stride + t/page_size] at place t % page_size; all layers share
+ * the table.  Pages of different sequences may be shared for reading. */
+typedef struct {
+  int type, n_layer, n_pages, page_size, n_kv, head_dim;
+  void *k, *v;
+} cwen_kv;
+/* Write row r of k (turned to pos[r], or to slot[r] with pos NULL; not turned
+ * with r NULL) and of v to slot[r] of sequence seq[r].  Rows are of the
+ * cache's type, or F32 and rounded once.  seq[r] < 0 skips the row (padding).
+ * Two rows of one call must not have the same place. */
+int cwen_cuda_kv_append(const cwen_kv *c, int layer, const int *table, int table_stride, int n_seq, int type,
+                        int n_rows, const void *k, int64_t krow, int64_t khead, const void *v, int64_t vrow,
+                        int64_t vhead, const int *seq, const int *slot, const cwen_rope *r, const int *pos,
+                        void *stream);
+/* Keep the accepted nodes of each sequence: the i-th set bit u of keep[s] moves
+ * slot len[s] + u to len[s] + i, K and V of every layer; len_out[s] (or NULL; not
+ * len itself) = len[s] + number of set bits.  Bitwise copies. */
+int cwen_cuda_kv_compact(const cwen_kv *c, const int *table, int table_stride, int n_seq, const int *len,
+                         const uint64_t *keep, int *len_out, void *stream);
+
+/* Causal attention over packed prompts: sequence s holds rows cu[s]..cu[s+1]-1
+ * (cu: n_seq + 1 non-decreasing row numbers on the device, at most n_rows) of q
+ * [n_head], k and v [n_kv] and out [n_head]; query head h reads kv head
+ * h / (n_head/n_kv).  out_i = sum_{j <= i} softmax(scale q_i.k_j) v_j.  Rows
+ * outside [cu[0], cu[n_seq]) are left as they were. */
+int cwen_cuda_attn_prompt(int type, int n_seq, const int *cu, int n_rows, int n_head, int n_kv, int head_dim,
+                          float scale, const void *q, int64_t qrow, int64_t qhead, const void *k, int64_t krow,
+                          int64_t khead, const void *v, int64_t vrow, int64_t vhead, void *out, int64_t orow,
+                          int64_t ohead, void *stream);
+
+/* Attention of drafted nodes over the cache.  Sequence s has len[s] committed
+ * slots and n_node[s] <= T <= 64 nodes (NULL: T; more or less count as T or 0)
+ * in slots len[s].. on; row s*T + t of q and out is its node t.  A node sees
+ * every committed slot and the nodes whose bit is set in mask[s*T + t] (NULL:
+ * nodes 0..t, a chain; T = 1 is single-token decode); a node that sees nothing
+ * gives zeros.  Rows t >= n_node[s] are left as they were.  max_len >= len[s] +
+ * n_node[s] for every s (the pages are not read beyond it).  ws is scratch of
+ * this call, cwen_cuda_attn_tree_ws bytes, 16-byte aligned, no contents kept:
+ * calls or graphs that may overlap need one each. */
+int cwen_cuda_attn_tree(const cwen_kv *c, int layer, const int *table, int table_stride, int n_seq, const int *len,
+                        int max_len, int T, const int *n_node, const uint64_t *mask, int n_head, float scale,
+                        const void *q, int64_t qrow, int64_t qhead, void *out, int64_t orow, int64_t ohead, void *ws,
+                        size_t ws_bytes, void *stream);
+size_t cwen_cuda_attn_tree_ws(const cwen_kv *c, int n_seq, int T, int n_head);
+/* Synchronize `stream` and report, then clear, what the operators met since the
+ * last status call: CWEN_OK, CWEN_ERANGE (an out-of-range sequence, slot,
+ * length or page id was left out) or CWEN_ETIMEOUT (a bounded device wait gave
+ * up: those outputs are not valid). */
+int cwen_cuda_attn_status(void *stream);
 
 /* ---- row sharding across the GPUs of one node (one engine per GPU) ----
  * The FFN matrices (ffn_gate, ffn_up, ffn_down) and the lm_head (output.weight)

@@ -7,51 +7,28 @@
 // First form: one warp per (row, head) with an online softmax over chunks of
 // 32 slots, one slot per lane for the scores, then one slice of dims per lane
 // for the weighted sum.
-#include "attnops.cuh"
+#include "attn_tc.cuh"
 
 namespace cw {
-
-struct AttnOp {
-  KvView kv;                 // tree
-  const void *k, *v;         // prompt
-  int64_t krow, khead, vrow, vhead;
-  const void *q;
-  int64_t qrow, qhead;
-  void *o;
-  int64_t orow, ohead;
-  const int *cu, *len, *n_node;
-  const uint64_t *mask;
-  int n_seq, n_rows, T, max_len, nh, nkv;
-  float scale;
-  int *err;
-};
 
 template <class T, int HD, bool TREE>
 __global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant__ AttnOp a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int DL = HD / 32;
-  __shared__ float qs[4][HD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + warp;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int64_t n_items = (int64_t)(TREE ? a.n_seq * a.T : a.n_rows) * a.nh;
   if (item >= n_items) return;
-  const int row = (int)(item / a.nh), h = (int)(item % a.nh), hk = h / (a.nh / a.nkv);
-  int s = 0, begin = 0, n, cap, t = 0, len = 0, live = 0;
-  uint64_t bits = 0;
+  const int row = (int)(item / a.nh), h = (int)(item % a.nh);
   if constexpr (TREE) {
-    s = row / a.T;
-    t = row % a.T;
-    live = a.n_node ? min(max(a.n_node[s], 0), a.T) : a.T;
-    if (t >= live) return;
-    len = a.len[s];
-    if (len < 0 || (int64_t)len + live > a.max_len) {
-      if (lane == 0) atomicOr(a.err, OPE_PAGE);
-      len = len < 0 ? 0 : len;
-    }
-    bits = a.mask ? a.mask[(int64_t)s * a.T + t] : (t == 63 ? ~0ull : (2ull << t) - 1);
-    n = (int)min((int64_t)len + live, (int64_t)a.max_len);
-    cap = 0;
+    const int s = row / a.T, t = row % a.T;
+    const TreeSeq q = tree_seq(a, s);
+    if (t >= q.live) return;
+    bool bad = q.cut;
+    for (int j = (threadIdx.x & 31) * a.kv.page_size; !bad && j < q.n; j += 32 * a.kv.page_size)
+      bad = cwp_row(a.kv.table + (int64_t)s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, j) < 0;
+    if (bad) atomicOr(a.err, OPE_PAGE);
+    __syncwarp();
+    exact_row<T, HD, true>(a, s, t, 0, row, h);
   } else {
     int lo = 0, hi = a.n_seq;  // the last sequence that begins at or before the row
     while (hi - lo > 1) {
@@ -59,65 +36,11 @@ __global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant_
       if (a.cu[mid] <= row) lo = mid;
       else hi = mid;
     }
-    begin = a.cu[lo];
-    if (begin < 0 || row < begin || row >= a.cu[lo + 1]) return;
-    n = row - begin + 1;
-    cap = n;
+    int b, e;
+    prompt_seq(a, lo, b, e);
+    if (row < b || row >= e) return;
+    exact_row<T, HD, false>(a, 0, 0, b, row, h);
   }
-  (void)cap;
-  const T *q = (const T *)a.q + row * a.qrow + h * a.qhead;
-  for (int d = lane; d < HD; d += 32) qs[warp][d] = to_f<T>(q[d]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, acc[DL];
-#pragma unroll
-  for (int i = 0; i < DL; i++) acc[i] = 0.f;
-  for (int c0 = 0; c0 < n; c0 += 32) {
-    const int j = c0 + lane;
-    bool see = j < n;
-    const T *kp = nullptr, *vp = nullptr;
-    if constexpr (TREE) {
-      if (see && j >= len) see = (bits >> (j - len)) & 1;
-      if (see) {
-        const int64_t r = cwp_row(a.kv.table + (int64_t)s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, j);
-        if (r < 0) {
-          atomicOr(a.err, OPE_PAGE);
-          see = false;
-        } else {
-          kp = (const T *)a.kv.k + (r * a.nkv + hk) * HD;
-          vp = (const T *)a.kv.v + (r * a.nkv + hk) * HD;
-        }
-      }
-    } else if (see) {
-      kp = (const T *)a.k + (begin + j) * a.krow + hk * a.khead;
-      vp = (const T *)a.v + (begin + j) * a.vrow + hk * a.vhead;
-    }
-    float sc = -INFINITY;
-    if (see) {
-      float d0 = 0.f;
-      for (int d = 0; d < HD; d++) d0 = fmaf(qs[warp][d], to_f<T>(kp[d]), d0);
-      sc = d0 * a.scale;
-    }
-    const float mn = fmaxf(m, warp_max(sc));
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float corr = m == -INFINITY ? 0.f : expf(m - ref);
-    const float e = see ? expf(sc - ref) : 0.f;
-    l = fmaf(l, corr, warp_sum(e));
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < DL; i++) acc[i] *= corr;
-    const unsigned live_m = __ballot_sync(0xffffffffu, see);
-    for (int t2 = 0; t2 < 32; t2++) {
-      if (!((live_m >> t2) & 1)) continue;
-      const float p = __shfl_sync(0xffffffffu, e, t2);
-      const T *vv = (const T *)__shfl_sync(0xffffffffu, (unsigned long long)vp, t2);
-#pragma unroll
-      for (int i = 0; i < DL; i++) acc[i] = fmaf(p, to_f<T>(vv[lane + 32 * i]), acc[i]);
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *o = (T *)a.o + row * a.orow + h * a.ohead;
-#pragma unroll
-  for (int i = 0; i < DL; i++) o[lane + 32 * i] = from_f<T>(l == 0.f ? 0.f : acc[i] * inv);
 }
 
 template <class T, bool TREE>
@@ -131,15 +54,20 @@ cudaError_t launch_simple(const AttnOp &a, int hd, cudaStream_t st) {
 template <bool TREE>
 cudaError_t launch_attn_op(const AttnOp &a, int type, int hd, cudaStream_t st) {
   if (type == CWEN_T_F32) return launch_simple<float, TREE>(a, hd, st);
-  if (type == CWEN_T_F16) return launch_simple<__half, TREE>(a, hd, st);
-  return launch_simple<__nv_bfloat16, TREE>(a, hd, st);
+  return TREE ? tc_tree(a, type == CWEN_T_BF16, hd, st) : tc_prompt(a, type == CWEN_T_BF16, hd, st);
 }
 
 static bool heads_ok(int nh, int nkv, int hd) {
   return nkv >= 1 && nkv <= 256 && nh >= nkv && nh <= 4096 && nh % nkv == 0 && (hd == 64 || hd == 128 || hd == 256);
 }
 
-cudaError_t attnops_configure() { return cudaSuccess; }
+// Rows of one part of a split row tile.
+static int part_rows(int T, int G) {
+  const int64_t n = (int64_t)T * G;
+  return n >= TC_ROWS ? TC_ROWS : (int)(n + 3) / 4 * 4;
+}
+
+cudaError_t attnops_configure() { return tc_configure(); }
 
 }  // namespace cw
 
@@ -175,8 +103,9 @@ int cwen_cuda_attn_prompt(int type, int n_seq, const int *cu, int n_rows, int n_
 }
 
 size_t cwen_cuda_attn_tree_ws(const cwen_kv *c, int n_seq, int T, int n_head) {
-  (void)n_seq; (void)T; (void)n_head;
-  return c ? 16 : 0;
+  (void)n_seq;  // the parts of a call are counted by CTAs, not by sequences
+  if (!c || T < 1 || n_head < 1 || c->n_kv < 1 || c->head_dim < 1) return 0;
+  return (size_t)TC_CTAS * 2 * part_rows(T, n_head / c->n_kv) * (c->head_dim + 2) * sizeof(float);
 }
 
 int cwen_cuda_attn_tree(const cwen_kv *c, int layer, const int *table, int table_stride, int n_seq, const int *len,
@@ -187,9 +116,9 @@ int cwen_cuda_attn_tree(const cwen_kv *c, int layer, const int *table, int table
   if (rc) return rc;
   if (layer < 0 || layer >= c->n_layer || !table || table_stride < 1 || n_seq < 0 || n_seq > 65535 || !len || T < 1 ||
       T > 64 || max_len < 1 || max_len > (1 << 30) || max_len > (int64_t)table_stride * c->page_size ||
-      !heads_ok(n_head, c->n_kv, c->head_dim) || !q || !out) {
+      !heads_ok(n_head, c->n_kv, c->head_dim) || kv_layer_rows(c) > 0x7fffffff || !q || !out) {
     set_error("cwen_cuda_attn_tree: need a layer of the cache, a table, 1 <= T <= 64, 1 <= max_len <= table_stride * "
-              "page_size, n_head a multiple of n_kv, head_dim 64, 128 or 256, non-null buffers");
+              "page_size, n_head a multiple of n_kv, head_dim 64, 128 or 256, fewer than 2^31 slots, non-null buffers");
     return CWEN_EINVAL;
   }
   if (!ws || ws_bytes < cwen_cuda_attn_tree_ws(c, n_seq, T, n_head) || (uintptr_t)ws % 16) {
@@ -212,6 +141,10 @@ int cwen_cuda_attn_tree(const cwen_kv *c, int layer, const int *table, int table
   a.q = q; a.qrow = qrow; a.qhead = qhead; a.o = out; a.orow = orow; a.ohead = ohead;
   a.len = len; a.n_node = n_node; a.mask = mask; a.n_seq = n_seq; a.T = T; a.max_len = max_len;
   a.nh = n_head; a.nkv = c->n_kv; a.scale = scale; a.err = E.op_err;
+  a.part_rows = part_rows(T, n_head / c->n_kv);
+  a.n_cta = E.n_sm < TC_CTAS ? E.n_sm : TC_CTAS;
+  a.part = (float *)ws;
+  a.ml = a.part + (size_t)TC_CTAS * 2 * a.part_rows * c->head_dim;
   CW_CHECK((launch_attn_op<true>(a, c->type, c->head_dim, stream ? (cudaStream_t)stream : E.stream)));
   E.prof.launches++;
   return CWEN_OK;

@@ -69,8 +69,30 @@ CW_DEV void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar) 
                : "memory");
 }
 
+// Tile of a tensor map (global -> shared through the TMA engine), completes on
+// an mbarrier.  x * element size a multiple of 16 bytes, dst 1024-byte aligned.
+CW_DEV void tma_3d(void *dst, const void *map, int x, int y, int z, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+// 16-byte asynchronous copy by this thread, or 16 zero bytes when !valid.
+CW_DEV void cp_async16(uint32_t dst, const void *src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+CW_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+CW_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Named barrier over `n` threads (id 1..15; 0 is __syncthreads).
 CW_DEV void named_bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+// The half that only arrives (its partners wait with named_bar).
+CW_DEV void named_bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // ---- 5th-generation tensor cores: tensor memory (TMEM) and tcgen05.mma ----
 // TMEM is 128 lanes x 512 columns of 32 bits per SM; an address is
@@ -129,6 +151,17 @@ CW_DEV void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+CW_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 CW_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor of a K-major operand without swizzle:
@@ -144,6 +177,28 @@ CW_DEV uint64_t smem_desc_kmajor(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
 // f32 accumulator: D format [4,6) = 1, N >> 3 at [17,23), M >> 4 at [24,29).
 constexpr uint32_t tc_idesc_f16(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// The same for operands with 128-byte swizzle (rows of 128 bytes, 8 rows per
+// 1024-byte atom, 16-byte unit u of row r at u ^ (r & 7); layout 2 at [61,64)).
+// K-major: rows are M or N, the next 8 rows `sbo` bytes on, the next 16 K
+// elements of the 64 in a row 32 bytes on; lbo is not used.  MN-major: rows are
+// K, the next 8 of them `sbo` bytes on, the next 64 M or N elements `lbo`.
+CW_DEV uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return smem_desc_kmajor(saddr, lbo, sbo) | (2ull << 61);
+}
+// Instruction descriptor of kind::f16 with A and B of one type (f16, or bf16:
+// formats 1 at [7,10) and [10,13)), B MN-major with b_mn (bit 16).
+constexpr uint32_t tc_idesc_16(bool bf16, bool b_mn, int M, int N) {
+  return tc_idesc_f16(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+// D[tmem] (+)= A[smem desc] * B[smem desc], issued by one thread.
+CW_DEV void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem desc], issued by one thread.  accumulate = 0
 // overwrites D.

@@ -1,5 +1,5 @@
-// Attention of f16 / bf16 rows on the 5th-generation tensor cores: causal
-// packed prompts, and drafted trees over a paged cache.
+// Attention on the 5th-generation tensor cores: causal packed prompts, and
+// drafted trees over a paged cache.
 //
 // A tile of 128 query rows (prompt: 128 tokens of one head; tree: the (node,
 // head) rows of one kv head) walks its slots in tiles of 128:
@@ -16,6 +16,15 @@
 // or warps 9-12 (tree, and prompts whose rows TMA cannot address) fill a ring of
 // 16 KB pieces in the order in which the MMAs use them: K as 128 slots x 64
 // dims, V as 8192/HD slots x HD dims, both with 128-byte swizzle.
+//
+// f32 rows are split in two f16 parts, x 2^e = hi + lo to 2^-22 of x, and every
+// product is hi hi + lo hi + hi lo (lo lo is below 2^-22 of it): three f16 MMAs
+// for one.  e is exact per row of Q; for K and V it comes from the largest
+// value of a window's first piece, with 2^7 to spare above it: what passes that
+// becomes infinite and goes the way of the last paragraph, what is small keeps
+// 2^-33 of that largest value.  The tensor cores add with truncation, which drifts
+// by up to 2^-24 of O per step of 16 slots, so O is taken out every WIN tiles and
+// added up in fp32 in the output (or part) rows.
 //
 // Rows that come out non-finite, and tiles that met a bad page id, are done
 // again by exact_row: a masked place must not reach a row even as 0 x NaN.
@@ -34,15 +43,25 @@ constexpr int PIECE = 16384;
 constexpr float P_SHIFT_F16 = 7.f;  // p <= 2^(8+7) < 65504
 constexpr float RESCALE_AT = 8.f;
 
-template <int HD>
+enum { TY_F32, TY_F16, TY_BF16 };
+template <int TY> struct TypeOf;
+template <> struct TypeOf<TY_F32> { using T = float; };
+template <> struct TypeOf<TY_F16> { using T = __half; };
+template <> struct TypeOf<TY_BF16> { using T = __nv_bfloat16; };
+
+template <int TY, int HD>
 struct Geo {
+  static constexpr bool F32 = TY == TY_F32;
   static constexpr int CB = HD / 64;         // 64-dim blocks of a row
-  static constexpr int Q_BYTES = CB * 16384; // [block][128 rows][128 B]
-  static constexpr int NP = CB;              // pieces of a K or a V tile
+  static constexpr int Q_BYTES = CB * 16384; // [block][128 rows][128 B]; f32: hi, then lo
+  static constexpr int NP = CB;              // pieces of a K or a V tile (f32: pairs of pieces)
   static constexpr int VK = 8192 / HD;       // slots of a V piece
-  static constexpr int NS = HD == 256 ? 9 : HD == 128 ? 11 : 12;
-  static constexpr int SMEM = Q_BYTES + NS * PIECE + 1024;
+  static constexpr int NS = F32 ? (HD == 256 ? 5 : HD == 128 ? 9 : 11) : (HD == 256 ? 9 : HD == 128 ? 11 : 12);
+  static constexpr int SMEM = Q_BYTES * (F32 ? 2 : 1) + NS * PIECE + 1024;
+  static constexpr int LOADERS = F32 ? 256 : 128;
+  static constexpr int threads(bool tma) { return tma ? 320 : 288 + LOADERS; }
 };
+constexpr int WIN = 4;  // f32: tiles of a window
 
 struct Ctl {
   uint64_t full[12], empty[12], s_full[2], p_ready[2], pv_done, q_full, o_free, o_done, drained;
@@ -55,11 +74,15 @@ struct Ctl {
   float mref[TC_ROWS];
   float2 ml[2][TC_ROWS];
   uint32_t rowoff[2][TC_KEYS];
+  // f32: exponents that Q rows, and a window's K and V, were multiplied by (the loaders run up to three windows ahead)
+  int qe[TC_ROWS], ke[8], ve[8];
+  float amax[8];
 };
 
-// Where one segment of work lies: the tiles [t0, t1) of a row tile's nt.
+// Where one segment of work lies: the tiles [w0, w1) of a row tile's nt, and
+// the window [t0, t1) of them at hand.
 struct Seg {
-  int s, hk, mt, t0, t1, nt;
+  int s, hk, mt, t0, t1, nt, w0, w1;
   TreeSeq ts;
 };
 
@@ -117,6 +140,22 @@ struct TreeWalk {
   }
 };
 
+// 2^e, e cut to the normal floats.
+CW_DEV float exp2_int(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+// The exponent that brings a largest value into [2^8, 2^9); 0 for zeros and non-finite ones.
+CW_DEV int scale_exp(float amax) {
+  if (!(amax > 1e-30f) || !(amax < INFINITY)) return 0;
+  return 8 - ((__float_as_int(amax) >> 23) - 127);
+}
+// Two floats as f16 hi and lo parts.
+CW_DEV void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *(const uint32_t *)&h;
+  lo = *(const uint32_t *)&l;
+}
+
 CW_DEV uint32_t pack2(bool bf, float lo, float hi) {
   uint32_t r;
   if (bf) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -136,25 +175,27 @@ CW_DEV uint32_t tree_word(const TreeSeq &q, uint64_t bits, int base) {
 
 }  // namespace
 
-template <bool BF, int HD, bool TREE, bool TMA>
-__global__ void __launch_bounds__(TMA ? 320 : 416, 1)
+template <int TY, int HD, bool TREE, bool TMA>
+__global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
     attn_tc_kernel(const __grid_constant__ AttnOp a, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv) {
-  using G_ = Geo<HD>;
-  using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
+  using G_ = Geo<TY, HD>;
+  using T = typename TypeOf<TY>::T;
+  constexpr bool F32 = TY == TY_F32, BF = TY == TY_BF16;
+  constexpr int LD = G_::LOADERS;
   constexpr int CB = G_::CB, NP = G_::NP, VK = G_::VK, NS = G_::NS;
   constexpr int O_COL = 0, S_COL = 256;
   __shared__ Ctl c;
   extern __shared__ uint8_t dyn[];
   uint8_t *qs = (uint8_t *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
-  uint8_t *ring = qs + G_::Q_BYTES;
+  uint8_t *ring = qs + G_::Q_BYTES * (F32 ? 2 : 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.nh / a.nkv;
 
   pdl_trigger();
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
-      mbar_init(&c.full[i], TMA ? 1 : 128);
+      mbar_init(&c.full[i], TMA ? 1 : LD);
       mbar_init(&c.empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -239,29 +280,42 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
   TreeWalk walk;
   if constexpr (TREE) walk.start(a, c);
   bool once = true;
+  int w_at = 0, w_end = 0;  // f32: what is left of the segment
   auto next = [&](Seg &g) -> bool {
-    if constexpr (TREE) {
-      return walk.next(a, g);
+    if (F32 && w_at < w_end) {
+      g.t0 = w_at;
     } else {
-      g.s = 0;
-      g.hk = ph / G;
-      g.mt = ptile;
-      g.t0 = 0;
-      g.t1 = g.nt = ptile + 1;
-      const bool r = once;
-      once = false;
-      return r;
+      if constexpr (TREE) {
+        if (!walk.next(a, g)) return false;
+      } else {
+        if (!once) return false;
+        once = false;
+        g.s = 0;
+        g.hk = ph / G;
+        g.mt = ptile;
+        g.t0 = 0;
+        g.t1 = g.nt = ptile + 1;
+      }
+      g.w0 = g.t0;
+      g.w1 = w_end = g.t1;
     }
+    if (F32) {
+      g.t1 = min(g.w1, g.t0 + WIN);
+      w_at = g.t1;
+    }
+    return true;
   };
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
     const int wg = warp >> 2, r = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const float sc = fabsf(a.scale) * 1.4426950408889634f;
+    float sc = fabsf(a.scale) * 1.4426950408889634f;
     constexpr float SHIFT = BF ? 0.f : P_SHIFT_F16;
-    const bool qvec = a.scale >= 0.f && ((uintptr_t)a.q % 16) == 0 && a.qrow % 8 == 0 && a.qhead % 8 == 0;
-    const bool ovec = ((uintptr_t)a.o % 16) == 0 && a.orow % 8 == 0 && a.ohead % 8 == 0;
+    constexpr int AL = 16 / sizeof(T);
+    const bool qvec = (F32 || a.scale >= 0.f) && ((uintptr_t)a.q % 16) == 0 && a.qrow % AL == 0 && a.qhead % AL == 0;
+    const bool ovec = ((uintptr_t)a.o % 16) == 0 && a.orow % AL == 0 && a.ohead % AL == 0;
+    float m_acc = -INFINITY, l_acc = 0.f;  // f32: of the windows so far
     int gt = 0;  // tiles of the CTA so far
     Seg g;
     for (int si = 0; next(g); si++) {
@@ -280,6 +334,8 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           return row < pend;
         }
       };
+      const bool first = g.t0 == g.w0, last = g.t1 == g.w1;  // window of the segment
+      if (first) {
       for (int i = tid; i < 128 * CB * 8; i += 256) {
         const int rr = i / (CB * 8), u = i % (CB * 8);
         int64_t row;
@@ -287,7 +343,29 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
         const bool have = place(rr, row, h, t);
         uint8_t *dst = qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4);
         const T *src = (const T *)a.q + (have ? row * a.qrow + h * a.qhead + u * 8 : 0);
-        if (qvec) {
+        if constexpr (F32) {
+          float x[8];
+          if (qvec && have) {
+            *(float4 *)x = *(const float4 *)src;
+            *(float4 *)(x + 4) = *(const float4 *)(src + 4);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = have ? src[k] : 0.f;
+          }
+          float mx = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
+#pragma unroll
+          for (int k = 1; k < CB * 8; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+          const int e = scale_exp(mx);
+          const float f = a.scale < 0.f ? -exp2_int(e) : exp2_int(e);
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) split2(x[2 * k] * f, x[2 * k + 1] * f, hi[k], lo[k]);
+          *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4 *)(dst + G_::Q_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (u == 0) c.qe[rr] = e;
+        } else if (qvec) {
           cp_async16(smem_u32(dst), src, have);
         } else {
           T e[8];
@@ -299,6 +377,7 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           *(uint4 *)dst = *(uint4 *)e;
         }
       }
+      }
       int64_t row;
       int h, t;
       const bool have = place(r, row, h, t);
@@ -306,10 +385,13 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
       if constexpr (TREE)
         if (have) bits = tree_bits(a, g.ts, g.s, t);
       const bool warp_live = __any_sync(0xffffffffu, have);
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      mbar_arrive(&c.q_full);
+      if (first) {
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        if (F32) named_bar(3, 256);  // qe
+        mbar_arrive(&c.q_full);
+      }
 
       const int nt = g.t1 - g.t0;
       float m_own = -INFINITY, l_own = 0.f;
@@ -319,6 +401,7 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
         const uint32_t S = tm + lane_base + S_COL + 128 * wg;
         wait(&c.s_full[wg], (gi >> 1) & 1);
         tc_fence_after();
+        if (F32) sc = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-c.qe[r]) * exp2_int(-c.ke[si & 7]);
         const int tile = g.t0 + j;
         const bool masked = TREE ? (tile + 1) * TC_KEYS > g.ts.len : tile == g.mt;
         auto word = [&](int k) -> uint32_t {
@@ -372,9 +455,10 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           m_own = m;
           const float mm = (m == -INFINITY ? 0.f : m) - SHIFT;
           float s0 = 0.f, s1 = 0.f;
+          uint32_t held[F32 ? 32 : 1];  // lo parts whose columns hold S yet
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            uint32_t x[32], p[16];
+            uint32_t x[32], p[16], q[F32 ? 16 : 1];
             tmem_ld32(S + 32 * k, x);
             tmem_wait_ld();
             const uint32_t w = word(k);
@@ -387,9 +471,28 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
               }
               s0 += p0;
               s1 += p1;
-              p[i >> 1] = pack2(BF, p0, p1);
+              if constexpr (F32) split2(p0, p1, p[i >> 1], q[i >> 1]);
+              else p[i >> 1] = pack2(BF, p0, p1);
             }
             tmem_st16(S + 16 * k, p);  // P over the S columns already read
+            if constexpr (F32) {       // lo parts at 64 + 16 k, once those are read too
+              if (k < 2) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) held[16 * k + i] = q[i];
+              } else {
+                if (k == 2) tmem_st32(S + 64, held);
+                else tmem_st16(S + 112, q);
+                if (k == 2) {
+#pragma unroll
+                  for (int i = 0; i < 16; i++) held[i] = q[i];
+                } else {
+                  uint32_t q2[16];
+#pragma unroll
+                  for (int i = 0; i < 16; i++) q2[i] = held[i];
+                  tmem_st16(S + 96, q2);
+                }
+              }
+            }
           }
           l_own += s0 + s1;
         }
@@ -410,16 +513,26 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
       }
       wait(&c.o_done, si & 1);
       tc_fence_after();
-      const bool whole = g.t0 == 0 && g.t1 == g.nt;
+      const bool whole = g.w0 == 0 && g.w1 == g.nt;
+      float f_old = 0.f, f_new = 1.f;  // f32: of the rows so far, of this window
+      if constexpr (F32) {
+        const float M = first ? m : fmaxf(m_acc, m);
+        f_old = first || m_acc == -INFINITY ? 0.f : ex2(m_acc - M);
+        f_new = m == -INFINITY ? 0.f : ex2(m - M);
+        l_acc = first ? l : l_acc * f_old + l * f_new;
+        m_acc = M;
+        l = l_acc;
+        f_new *= exp2_int(-c.ve[si & 7]);
+      }
       bool bad = c.bad || !(l < INFINITY);
-      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      const float inv = whole && last ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
       float *part = nullptr;
       if constexpr (TREE) {
         if (!whole) {
-          const int64_t pr = ((int64_t)blockIdx.x * 2 + (g.t0 == 0)) * a.part_rows + r;
+          const int64_t pr = ((int64_t)blockIdx.x * 2 + (g.w0 == 0)) * a.part_rows + r;
           part = a.part + pr * HD;
-          if (have && wg == 0) {
-            a.ml[2 * pr] = m;
+          if (have && wg == 0 && last) {
+            a.ml[2 * pr] = F32 ? m_acc : m;
             a.ml[2 * pr + 1] = c.bad ? __int_as_float(0x7fffffff) : l;
           }
         }
@@ -432,19 +545,41 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           tmem_ld32(tm + lane_base + O_COL + col, x);
           tmem_wait_ld();
           if (!have) continue;
-          float f[32];
+          T *o = (T *)a.o + row * a.orow + h * a.ohead + col;
+          if constexpr (F32) {
+            float *dst = part ? part + col : (float *)o;
+            const bool v4 = part || ovec;
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            f[i] = l == 0.f ? 0.f : __uint_as_float(x[i]) * inv;
-            bad |= !(fabsf(f[i]) < INFINITY);
-          }
-          if (TREE && part) {
+            for (int i = 0; i < 32; i += 4) {
+              float old[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+              if (!first) {
+                if (v4) *(float4 *)old = *(const float4 *)(dst + i);
+                else
+                  for (int d = 0; d < 4; d++) old[d] = dst[i + d];
+              }
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *(float4 *)(part + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+              for (int d = 0; d < 4; d++) {
+                f[d] = __uint_as_float(x[i + d]) * f_new;
+                if (!first) f[d] = fmaf(old[d], f_old, f[d]);
+                f[d] = l == 0.f ? 0.f : f[d] * inv;
+                bad |= !(fabsf(f[d]) < INFINITY);
+              }
+              if (v4) *(float4 *)(dst + i) = *(const float4 *)f;
+              else
+                for (int d = 0; d < 4; d++) dst[i + d] = f[d];
+            }
           } else {
-            T *o = (T *)a.o + row * a.orow + h * a.ohead + col;
-            if (ovec) {
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+              f[i] = l == 0.f ? 0.f : __uint_as_float(x[i]) * inv;
+              bad |= !(fabsf(f[i]) < INFINITY);
+            }
+            if (TREE && part) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *(float4 *)(part + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            } else if (ovec) {
 #pragma unroll
               for (int i = 0; i < 32; i += 8)
                 *(uint4 *)(o + i) = make_uint4(pack2(BF, f[i], f[i + 1]), pack2(BF, f[i + 2], f[i + 3]),
@@ -456,7 +591,7 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           }
         }
       }
-      if (have && bad && whole) atomicOr(&c.badrows[r >> 5], 1u << (r & 31));
+      if (have && bad && whole && last) atomicOr(&c.badrows[r >> 5], 1u << (r & 31));
       tc_fence_before();
       mbar_arrive(&c.o_free);
       named_bar(3, 256);
@@ -494,21 +629,33 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
       };
       auto qk = [&](int gi) {
         const uint32_t d = tm + S_COL + 128 * (gi & 1);
-        for (int b = 0; b < NP; b++) {
-          take();
+        auto block = [&](uint32_t q, bool add) {
 #pragma unroll
           for (int k = 0; k < 4; k++)
-            tc_mma_ss(d, smem_desc_sw128(q0 + b * 16384 + k * 32, 16, 1024),
-                      smem_desc_sw128(r0 + slot * PIECE + k * 32, 16, 1024), I_S, (b | k) != 0);
+            tc_mma_ss(d, smem_desc_sw128(q + k * 32, 16, 1024), smem_desc_sw128(r0 + slot * PIECE + k * 32, 16, 1024), I_S,
+                      add || k);
+        };
+        for (int b = 0; b < NP; b++) {
+          take();
+          block(q0 + b * 16384, b != 0);
+          if (F32) block(q0 + G_::Q_BYTES + b * 16384, true);
           give();
+          if (F32) {
+            take();
+            block(q0 + b * 16384, true);
+            give();
+          }
         }
         tc_commit(&c.s_full[gi & 1]);
       };
       Seg g;
+      int qi = 0;
       for (int si = 0; next(g); si++) {
         const int nt = g.t1 - g.t0;
-        wait(&c.q_full, si & 1);
-        tc_fence_after();
+        if (g.t0 == g.w0) {
+          wait(&c.q_full, qi++ & 1);
+          tc_fence_after();
+        }
         qk(gt);
         if (nt > 1) qk(gt + 1);
         if (si > 0) {
@@ -520,13 +667,22 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
           wait(&c.p_ready[gi & 1], (gi >> 1) & 1);
           tc_fence_after();
           const uint32_t p = tm + S_COL + 128 * (gi & 1);
-          for (int b = 0; b < NP; b++) {
-            take();
+          auto block = [&](uint32_t pb, bool add) {
 #pragma unroll
             for (int k = 0; k < VK / 16; k++)
-              tc_mma_ts(tm + O_COL, p + (b * (VK / 16) + k) * 8,
-                        smem_desc_sw128(r0 + slot * PIECE + k * 2048, VK * 128, 1024), I_O, (j | b | k) != 0);
+              tc_mma_ts(tm + O_COL, pb + k * 8, smem_desc_sw128(r0 + slot * PIECE + k * 2048, VK * 128, 1024), I_O, add || k);
+          };
+          for (int b = 0; b < NP; b++) {
+            const uint32_t pb = p + b * (VK / 16) * 8;
+            take();
+            block(pb, (j | b) != 0);
+            if (F32) block(pb + 64, true);
             give();
+            if (F32) {
+              take();
+              block(pb, true);
+              give();
+            }
           }
           tc_commit(&c.pv_done);
           if (j + 2 < nt) qk(gi + 2);
@@ -577,96 +733,210 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ loads, one 16-byte unit per thread
-    const int lt = tid - 288;  // 0..127
-    constexpr int D = 5;       // pieces in flight per thread
-    static_assert(D < NS, "a piece in flight needs its slot");
-    int slot = 0, par = 1, done = 0, issued = 0;
-    auto finish = [&]() {  // this thread's part of the oldest piece in flight has landed
-      fence_proxy_async_smem();
-      mbar_arrive(&c.full[done % NS]);
-      done++;
+    const int lt = tid - 288;
+    // piece `b` of tile `tile`: unit x (of 1024: 8 dims of a slot) -> slot of the tile, unit of the row, place in a piece
+    auto unit = [&](bool is_v, int b, int x, int &key, int &u) -> uint32_t {
+      if (!is_v) {
+        key = x >> 3;
+        u = b * 8 + (x & 7);
+        return key * 128 + (((x & 7) ^ (key & 7)) << 4);
+      }
+      constexpr int UR = HD / 8;  // units of a row
+      const int kr = x / UR;
+      u = x % UR;
+      key = b * VK + kr;
+      return (u >> 3) * (VK * 128) + kr * 128 + (((u & 7) ^ (kr & 7)) << 4);
     };
-    auto put = [&](bool is_v, int tile, int b, int hk) {
-      wait(&c.empty[slot], par);
-      const uint32_t base = smem_u32(ring + slot * PIECE);
-      const uint32_t *off = c.rowoff[tile & 1];
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        int key, u;         // slot of the tile, 16-byte unit of the row
-        uint32_t dst;
-        if (!is_v) {
-          key = (lt >> 3) + 16 * i;
-          u = b * 8 + (lt & 7);
-          dst = base + key * 128 + (((lt & 7) ^ (key & 7)) << 4);
-        } else {
-          constexpr int UR = HD / 8;  // units of a row
-          const int x = lt + 128 * i, kr = x / UR;
-          u = x % UR;
-          key = b * VK + kr;
-          dst = base + (u >> 3) * (VK * 128) + kr * 128 + (((u & 7) ^ (kr & 7)) << 4);
-        }
-        const uint32_t o = off[key];
-        const bool ok = o != 0xffffffffu;
-        const T *src;
+    auto source = [&](bool is_v, uint32_t o, int hk, int u) -> const T * {
+      if constexpr (TREE) return (const T *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + hk) * HD + u * 8;
+      return (const T *)(is_v ? a.v : a.k) + (int64_t)o * (is_v ? a.vrow : a.krow) + hk * (is_v ? a.vhead : a.khead) + u * 8;
+    };
+    constexpr uint32_t NONE = 0xffffffffu;
+    // pool rows (or prompt rows) of a tile's slots
+    auto offsets = [&](const Seg &g, int tile) {
+      named_bar(4, LD);  // the readers of two tiles ago are through
+      const int sl = tile * TC_KEYS + lt;
+      if (lt < TC_KEYS) {
+        uint32_t o = NONE;
         if constexpr (TREE) {
-          src = (const T *)(is_v ? a.kv.v : a.kv.k) + (ok ? ((int64_t)o * a.nkv + hk) * HD + u * 8 : 0);
-        } else {
-          src = (const T *)(is_v ? a.v : a.k) +
-                (ok ? (int64_t)o * (is_v ? a.vrow : a.krow) + hk * (is_v ? a.vhead : a.khead) + u * 8 : 0);
+          if (sl < g.ts.n) {
+            const int64_t x = cwp_row(a.kv.table + (int64_t)g.s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, sl);
+            if (x >= 0) {
+              o = (uint32_t)x;
+            } else {
+              c.bad = 1;
+              atomicOr(a.err, OPE_PAGE);
+            }
+          }
+          if (g.ts.cut && lt == 0) atomicOr(a.err, OPE_PAGE);
+        } else if (pbegin + sl < pend) {
+          o = (uint32_t)(pbegin + sl);
         }
-        if (TREE || a.vec) {
-          cp_async16(dst, src, ok);
+        c.rowoff[tile & 1][lt] = o;
+      }
+      named_bar(4, LD);
+    };
+    // the pieces in the order of their use: K(t0), then K(j), V(j - 1), then V(t1 - 1)
+    Seg g;
+    int si = -1, pj = 0, pb = 0;
+    bool is_v = false, more = false;
+    auto advance = [&]() -> bool {
+      if (more && ++pb == NP) {
+        pb = 0;
+        if (!is_v && pj > g.t0) {
+          is_v = true;
         } else {
-          T e[8];
-#pragma unroll
-          for (int k = 0; k < 8; k++) e[k] = ok ? src[k] : from_f<T>(0.f);
-          const uint4 w = *(uint4 *)e;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                       : "memory");
+          is_v = ++pj == g.t1;
+          more = pj <= g.t1;
         }
       }
-      cp_async_commit();
-      issued++;
+      if (!more) {
+        if (!next(g)) return false;
+        si++;
+        pj = g.t0;
+        pb = 0;
+        is_v = false;
+        more = true;
+      }
+      if (!is_v && pb == 0) offsets(g, pj);
+      return true;
+    };
+    int slot = 0, par = 1;  // the first pass over the ring waits for nothing
+    auto step = [&]() {
       if (++slot == NS) {
         slot = 0;
         par ^= 1;
       }
-      if (issued - done > D) {
-        cp_async_wait<D>();
-        finish();
-      }
     };
-    Seg g;
-    while (next(g)) {
-      for (int j = g.t0; j <= g.t1; j++) {
-        if (j < g.t1) {
-          named_bar(4, 128);  // both parities' readers of two tiles ago are through
-          const int sl = j * TC_KEYS + lt;
-          uint32_t o = 0xffffffffu;
-          if constexpr (TREE) {
-            if (sl < g.ts.n) {
-              const int64_t x = cwp_row(a.kv.table + (int64_t)g.s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, sl);
-              if (x >= 0) {
-                o = (uint32_t)x;
-              } else {
-                c.bad = 1;
-                atomicOr(a.err, OPE_PAGE);
-              }
+    if constexpr (F32) {
+      // registers hold the next piece while this one is split and stored
+      struct Piece {
+        float x[4][8];
+        bool v, first;
+        int b, si;
+      };
+      auto fetch = [&](Piece &p) {
+        p.v = is_v;
+        p.b = pb;
+        p.si = si;
+        const int tile = is_v ? pj - 1 : pj;
+        p.first = tile == g.t0 && pb == 0;
+        const bool vec = TREE || a.vec;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          int key, u;
+          unit(is_v, pb, lt + 256 * i, key, u);
+          const uint32_t o = c.rowoff[tile & 1][key];
+          if (o == NONE) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) p.x[i][k] = 0.f;
+          } else {
+            const float *src = (const float *)source(is_v, o, g.hk, u);
+            if (vec) {
+              *(float4 *)p.x[i] = *(const float4 *)src;
+              *(float4 *)(p.x[i] + 4) = *(const float4 *)(src + 4);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; k++) p.x[i][k] = src[k];
             }
-            if (g.ts.cut && lt == 0) atomicOr(a.err, OPE_PAGE);
-          } else if (pbegin + sl < pend) {
-            o = (uint32_t)(pbegin + sl);
           }
-          c.rowoff[j & 1][lt] = o;
-          named_bar(4, 128);
-          for (int b = 0; b < NP; b++) put(false, j, b, g.hk);
         }
-        if (j > g.t0)
-          for (int b = 0; b < NP; b++) put(true, j - 1, b, g.hk);
+      };
+      float fk = 1.f, fv = 1.f;
+      int es = 0;
+      auto store = [&](const Piece &p) {
+        if (p.first) {
+          float mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(p.x[i][k]));
+          mx = warp_max(mx);
+          named_bar(4, LD);
+          if (lane == 0) c.amax[warp - 9] = mx;
+          named_bar(4, LD);
+#pragma unroll
+          for (int i = 0; i < 8; i++) mx = fmaxf(mx, c.amax[i]);
+          const int e = scale_exp(mx);
+          (p.v ? fv : fk) = exp2_int(e);
+          es = e;
+        }
+        const float f = p.v ? fv : fk;
+        const int s_hi = slot;
+        wait(&c.empty[slot], par);
+        step();
+        const int s_lo = slot;
+        wait(&c.empty[slot], par);
+        step();
+        if (p.first && lt == 0) (p.v ? c.ve : c.ke)[p.si & 7] = es;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          int key, u;
+          const uint32_t at = unit(p.v, p.b, lt + 256 * i, key, u);
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) split2(p.x[i][2 * k] * f, p.x[i][2 * k + 1] * f, hi[k], lo[k]);
+          *(uint4 *)(ring + s_hi * PIECE + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4 *)(ring + s_lo * PIECE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&c.full[s_hi]);
+        mbar_arrive(&c.full[s_lo]);
+      };
+      Piece A, B;
+      bool have = advance();
+      if (have) fetch(A);
+      while (have) {
+        have = advance();
+        if (have) fetch(B);
+        store(A);
+        if (!have) break;
+        have = advance();
+        if (have) fetch(A);
+        store(B);
       }
+    } else {
+      constexpr int D = 5;  // pieces in flight per thread
+      static_assert(D < NS, "a piece in flight needs its slot");
+      int done = 0, issued = 0;
+      auto finish = [&]() {  // this thread's part of the oldest piece in flight has landed
+        fence_proxy_async_smem();
+        mbar_arrive(&c.full[done % NS]);
+        done++;
+      };
+      while (advance()) {
+        wait(&c.empty[slot], par);
+        const uint32_t base = smem_u32(ring + slot * PIECE);
+        const uint32_t *off = c.rowoff[(is_v ? pj - 1 : pj) & 1];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          int key, u;
+          const uint32_t dst = base + unit(is_v, pb, lt + 128 * i, key, u);
+          const uint32_t o = off[key];
+          const bool ok = o != NONE;
+          const T *src = source(is_v, ok ? o : 0, g.hk, u);
+          if (TREE || a.vec) {
+            cp_async16(dst, src, ok);
+          } else {
+            T e[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) e[k] = ok ? src[k] : from_f<T>(0.f);
+            const uint4 w = *(uint4 *)e;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                         : "memory");
+          }
+        }
+        cp_async_commit();
+        issued++;
+        step();
+        if (issued - done > D) {
+          cp_async_wait<D>();
+          finish();
+        }
+      }
+      cp_async_wait<0>();
+      while (done < issued) finish();
     }
-    cp_async_wait<0>();
-    while (done < issued) finish();
   }
   tc_fence_before();
   __syncthreads();
@@ -678,9 +948,9 @@ __global__ void __launch_bounds__(TMA ? 320 : 416, 1)
 
 // Joins the parts of a row whose slots were split over CTAs: one warp per row,
 // parts in CTA order.  Grid (sequence, kv head, groups of 8 rows).
-template <bool BF, int HD>
+template <int TY, int HD>
 __global__ void __launch_bounds__(256) tc_combine_kernel(const __grid_constant__ AttnOp a) {
-  using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
+  using T = typename TypeOf<TY>::T;
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, s = blockIdx.x, hk = blockIdx.y, G = a.nh / a.nkv;
@@ -775,36 +1045,60 @@ bool make_map(CUtensorMap *m, bool bf16, const void *p, int64_t row, int64_t hea
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool BF, int HD>
+template <int TY, int HD, bool TREE, bool TMA>
+cudaError_t configure_one() {
+  return cudaFuncSetAttribute(attn_tc_kernel<TY, HD, TREE, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Geo<TY, HD>::SMEM);
+}
+template <int TY, int HD>
 cudaError_t configure_hd() {
-  CW_TRY(cudaFuncSetAttribute(attn_tc_kernel<BF, HD, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<HD>::SMEM));
-  CW_TRY(cudaFuncSetAttribute(attn_tc_kernel<BF, HD, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<HD>::SMEM));
-  CW_TRY(cudaFuncSetAttribute(attn_tc_kernel<BF, HD, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<HD>::SMEM));
-  return carveout_max(tc_combine_kernel<BF, HD>);
+  if constexpr (TY != TY_F32) CW_TRY((configure_one<TY, HD, false, true>()));
+  CW_TRY((configure_one<TY, HD, false, false>()));
+  CW_TRY((configure_one<TY, HD, true, false>()));
+  return carveout_max(tc_combine_kernel<TY, HD>);
 }
 
-template <bool BF, int HD>
+template <int TY, int HD>
 cudaError_t prompt_hd(AttnOp a, cudaStream_t st) {
   CUtensorMap mk, mv;
   const int64_t tiles = (int64_t)a.n_rows / TC_ROWS + a.n_seq;
   if (tiles * a.nh > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)(tiles * a.nh));
-  if (make_map(&mk, BF, a.k, a.krow, a.khead, HD, a.nkv, a.n_rows, TC_KEYS) &&
-      make_map(&mv, BF, a.v, a.vrow, a.vhead, HD, a.nkv, a.n_rows, Geo<HD>::VK))
-    return launch_pdl(attn_tc_kernel<BF, HD, false, true>, grid, 320, Geo<HD>::SMEM, st, a, mk, mv);
+  using G = Geo<TY, HD>;
+  if constexpr (TY != TY_F32) {
+    if (make_map(&mk, TY == TY_BF16, a.k, a.krow, a.khead, HD, a.nkv, a.n_rows, TC_KEYS) &&
+        make_map(&mv, TY == TY_BF16, a.v, a.vrow, a.vhead, HD, a.nkv, a.n_rows, G::VK))
+      return launch_pdl(attn_tc_kernel<TY, HD, false, true>, grid, G::threads(true), G::SMEM, st, a, mk, mv);
+  }
   memset(&mk, 0, sizeof mk);
   memset(&mv, 0, sizeof mv);
-  a.vec = ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.krow | a.khead | a.vrow | a.vhead) % 8 == 0;
-  return launch_pdl(attn_tc_kernel<BF, HD, false, false>, grid, 416, Geo<HD>::SMEM, st, a, mk, mv);
+  const int al = TY == TY_F32 ? 4 : 8;
+  a.vec = ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.krow | a.khead | a.vrow | a.vhead) % al == 0;
+  return launch_pdl(attn_tc_kernel<TY, HD, false, false>, grid, G::threads(false), G::SMEM, st, a, mk, mv);
 }
 
-template <bool BF, int HD>
+template <int TY, int HD>
 cudaError_t tree_hd(const AttnOp &a, cudaStream_t st) {
   static const CUtensorMap none = {};
-  CW_TRY(launch_pdl(attn_tc_kernel<BF, HD, true, false>, dim3(a.n_cta), 416, Geo<HD>::SMEM, st, a, none, none));
+  using G = Geo<TY, HD>;
+  CW_TRY(launch_pdl(attn_tc_kernel<TY, HD, true, false>, dim3(a.n_cta), G::threads(false), G::SMEM, st, a, none, none));
   if (tree_tiles(a.max_len) == 1) return cudaSuccess;  // no segment can be split
-  const int G = a.nh / a.nkv;
-  return launch_pdl(tc_combine_kernel<BF, HD>, dim3(a.n_seq, a.nkv, (a.T * G + 7) / 8), 256, 0, st, a);
+  return launch_pdl(tc_combine_kernel<TY, HD>, dim3(a.n_seq, a.nkv, (a.T * (a.nh / a.nkv) + 7) / 8), 256, 0, st, a);
+}
+
+template <int TY>
+cudaError_t configure_ty() {
+  CW_TRY((configure_hd<TY, 64>()));
+  CW_TRY((configure_hd<TY, 128>()));
+  return configure_hd<TY, 256>();
+}
+template <int TY>
+cudaError_t prompt_ty(const AttnOp &a, int hd, cudaStream_t st) {
+  return hd == 64 ? prompt_hd<TY, 64>(a, st) : hd == 128 ? prompt_hd<TY, 128>(a, st) : prompt_hd<TY, 256>(a, st);
+}
+template <int TY>
+cudaError_t tree_ty(const AttnOp &a, int hd, cudaStream_t st) {
+  return hd == 64 ? tree_hd<TY, 64>(a, st) : hd == 128 ? tree_hd<TY, 128>(a, st) : tree_hd<TY, 256>(a, st);
 }
 
 }  // namespace
@@ -814,21 +1108,18 @@ cudaError_t tc_configure() {
   cudaDriverEntryPointQueryResult found;
   CW_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
   if (found == cudaDriverEntryPointSuccess) g_encode = (EncodeTiled)fn;
-  CW_TRY((configure_hd<true, 64>()));
-  CW_TRY((configure_hd<true, 128>()));
-  CW_TRY((configure_hd<true, 256>()));
-  CW_TRY((configure_hd<false, 64>()));
-  CW_TRY((configure_hd<false, 128>()));
-  return configure_hd<false, 256>();
+  CW_TRY(configure_ty<TY_F32>());
+  CW_TRY(configure_ty<TY_F16>());
+  return configure_ty<TY_BF16>();
 }
 
-cudaError_t tc_prompt(const AttnOp &a, bool bf16, int hd, cudaStream_t st) {
-  if (bf16) return hd == 64 ? prompt_hd<true, 64>(a, st) : hd == 128 ? prompt_hd<true, 128>(a, st) : prompt_hd<true, 256>(a, st);
-  return hd == 64 ? prompt_hd<false, 64>(a, st) : hd == 128 ? prompt_hd<false, 128>(a, st) : prompt_hd<false, 256>(a, st);
+cudaError_t tc_prompt(const AttnOp &a, int type, int hd, cudaStream_t st) {
+  if (type == CWEN_T_F32) return prompt_ty<TY_F32>(a, hd, st);
+  return type == CWEN_T_F16 ? prompt_ty<TY_F16>(a, hd, st) : prompt_ty<TY_BF16>(a, hd, st);
 }
-cudaError_t tc_tree(const AttnOp &a, bool bf16, int hd, cudaStream_t st) {
-  if (bf16) return hd == 64 ? tree_hd<true, 64>(a, st) : hd == 128 ? tree_hd<true, 128>(a, st) : tree_hd<true, 256>(a, st);
-  return hd == 64 ? tree_hd<false, 64>(a, st) : hd == 128 ? tree_hd<false, 128>(a, st) : tree_hd<false, 256>(a, st);
+cudaError_t tc_tree(const AttnOp &a, int type, int hd, cudaStream_t st) {
+  if (type == CWEN_T_F32) return tree_ty<TY_F32>(a, hd, st);
+  return type == CWEN_T_F16 ? tree_ty<TY_F16>(a, hd, st) : tree_ty<TY_BF16>(a, hd, st);
 }
 
 }  // namespace cw

@@ -1,4 +1,4 @@
-// Tensor-core attention for f16 and bf16 -- host interface (attn_tc.cu).
+// Tensor-core attention -- host interface (attn_tc.cu).
 #pragma once
 #include "attnops_dev.cuh"
 
@@ -8,7 +8,7 @@ namespace cw {
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_CTAS = 148;
 
 cudaError_t tc_configure();
-cudaError_t tc_prompt(const AttnOp &a, bool bf16, int hd, cudaStream_t st);
-cudaError_t tc_tree(const AttnOp &a, bool bf16, int hd, cudaStream_t st);
+cudaError_t tc_prompt(const AttnOp &a, int type, int hd, cudaStream_t st);
+cudaError_t tc_tree(const AttnOp &a, int type, int hd, cudaStream_t st);
 
 }  // namespace cw

@@ -1,61 +1,8 @@
-// Attention over packed prompts and over drafted trees on a paged cache.
-//
-//   o = sum_j p_j v_j,  p_j = exp(scale q.k_j - m) / sum, over the slots j the
-// row sees: j <= i inside its sequence (prompt), or the committed slots and
-// the nodes of its mask (tree).  A row that sees nothing gives zeros.
-//
-// First form: one warp per (row, head) with an online softmax over chunks of
-// 32 slots, one slot per lane for the scores, then one slice of dims per lane
-// for the weighted sum.
+// Attention over packed prompts and over drafted trees on a paged cache: the C
+// ABI (include/cwen_cuda.h).  The kernels are in attn_tc.cu.
 #include "attn_tc.cuh"
 
 namespace cw {
-
-template <class T, int HD, bool TREE>
-__global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant__ AttnOp a) {
-  pdl_trigger();
-  pdl_wait();
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t n_items = (int64_t)(TREE ? a.n_seq * a.T : a.n_rows) * a.nh;
-  if (item >= n_items) return;
-  const int row = (int)(item / a.nh), h = (int)(item % a.nh);
-  if constexpr (TREE) {
-    const int s = row / a.T, t = row % a.T;
-    const TreeSeq q = tree_seq(a, s);
-    if (t >= q.live) return;
-    bool bad = q.cut;
-    for (int j = (threadIdx.x & 31) * a.kv.page_size; !bad && j < q.n; j += 32 * a.kv.page_size)
-      bad = cwp_row(a.kv.table + (int64_t)s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, j) < 0;
-    if (bad) atomicOr(a.err, OPE_PAGE);
-    __syncwarp();
-    exact_row<T, HD, true>(a, s, t, 0, row, h);
-  } else {
-    int lo = 0, hi = a.n_seq;  // the last sequence that begins at or before the row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    int b, e;
-    prompt_seq(a, lo, b, e);
-    if (row < b || row >= e) return;
-    exact_row<T, HD, false>(a, 0, 0, b, row, h);
-  }
-}
-
-template <class T, bool TREE>
-cudaError_t launch_simple(const AttnOp &a, int hd, cudaStream_t st) {
-  const int64_t items = (int64_t)(TREE ? a.n_seq * a.T : a.n_rows) * a.nh;
-  const dim3 grid((unsigned)((items + 3) / 4));
-  if (hd == 64) return launch_pdl(attn_simple_kernel<T, 64, TREE>, grid, 128, 0, st, a);
-  if (hd == 128) return launch_pdl(attn_simple_kernel<T, 128, TREE>, grid, 128, 0, st, a);
-  return launch_pdl(attn_simple_kernel<T, 256, TREE>, grid, 128, 0, st, a);
-}
-template <bool TREE>
-cudaError_t launch_attn_op(const AttnOp &a, int type, int hd, cudaStream_t st) {
-  if (type == CWEN_T_F32) return launch_simple<float, TREE>(a, hd, st);
-  return TREE ? tc_tree(a, type == CWEN_T_BF16, hd, st) : tc_prompt(a, type == CWEN_T_BF16, hd, st);
-}
 
 static bool heads_ok(int nh, int nkv, int hd) {
   return nkv >= 1 && nkv <= 256 && nh >= nkv && nh <= 4096 && nh % nkv == 0 && (hd == 64 || hd == 128 || hd == 256);
@@ -97,7 +44,7 @@ int cwen_cuda_attn_prompt(int type, int n_seq, const int *cu, int n_rows, int n_
   a.k = k; a.v = v; a.krow = krow; a.khead = khead; a.vrow = vrow; a.vhead = vhead;
   a.q = q; a.qrow = qrow; a.qhead = qhead; a.o = out; a.orow = orow; a.ohead = ohead;
   a.cu = cu; a.n_seq = n_seq; a.n_rows = n_rows; a.nh = n_head; a.nkv = n_kv; a.scale = scale; a.err = E.op_err;
-  CW_CHECK((launch_attn_op<false>(a, type, head_dim, stream ? (cudaStream_t)stream : E.stream)));
+  CW_CHECK(tc_prompt(a, type, head_dim, stream ? (cudaStream_t)stream : E.stream));
   E.prof.launches++;
   return CWEN_OK;
 }
@@ -145,7 +92,7 @@ int cwen_cuda_attn_tree(const cwen_kv *c, int layer, const int *table, int table
   a.n_cta = E.n_sm < TC_CTAS ? E.n_sm : TC_CTAS;
   a.part = (float *)ws;
   a.ml = a.part + (size_t)TC_CTAS * 2 * a.part_rows * c->head_dim;
-  CW_CHECK((launch_attn_op<true>(a, c->type, c->head_dim, stream ? (cudaStream_t)stream : E.stream)));
+  CW_CHECK(tc_tree(a, c->type, c->head_dim, stream ? (cudaStream_t)stream : E.stream));
   E.prof.launches++;
   return CWEN_OK;
 }

@@ -40,6 +40,7 @@ namespace cw {
 namespace {
 
 constexpr int PIECE = 16384;
+constexpr int TMA_WARPS = 3;
 constexpr float P_SHIFT_F16 = 7.f;  // p <= 2^(8+7) < 65504
 constexpr float RESCALE_AT = 8.f;
 
@@ -59,7 +60,7 @@ struct Geo {
   static constexpr int NS = F32 ? (HD == 256 ? 5 : HD == 128 ? 9 : 11) : (HD == 256 ? 9 : HD == 128 ? 11 : 12);
   static constexpr int SMEM = Q_BYTES * (F32 ? 2 : 1) + NS * PIECE + 1024;
   static constexpr int LOADERS = F32 ? 256 : 128;
-  static constexpr int threads(bool tma) { return tma ? 320 : 288 + LOADERS; }
+  static constexpr int threads(bool tma) { return 288 + (tma ? 32 * TMA_WARPS : LOADERS); }
 };
 constexpr int WIN = 4;  // f32: tiles of a window
 
@@ -161,6 +162,44 @@ CW_DEV uint32_t pack2(bool bf, float lo, float hi) {
   if (bf) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Maximum of 32 scores over the slots of w.
+CW_DEV float max32(const uint32_t (&x)[32], uint32_t w, float mx) {
+  float m0 = mx, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+  if (w == ~0u) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      m0 = fmaxf(m0, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+      m1 = fmaxf(m1, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+      m2 = fmaxf(m2, fmaxf(__uint_as_float(x[i + 4]), __uint_as_float(x[i + 5])));
+      m3 = fmaxf(m3, fmaxf(__uint_as_float(x[i + 6]), __uint_as_float(x[i + 7])));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; i++) m0 = (w >> i) & 1 ? fmaxf(m0, __uint_as_float(x[i])) : m0;
+  }
+  return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+}
+// p = exp2(c s - m) of 32 scores, 0 outside w: as pairs of 16 bits (f32: hi and lo parts), and added to sum.
+template <bool F32, bool BF>
+CW_DEV void exp32(const uint32_t (&x)[32], uint32_t w, float sc, float mm, uint64_t &sum, uint32_t (&p)[16],
+                  uint32_t (&q)[F32 ? 16 : 1]) {
+  const uint64_t c2 = pack_f2(sc, sc), m2 = pack_f2(-mm, -mm);
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float a, b;
+    unpack_f2(fma_f2(pack_f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), c2, m2), a, b);
+    a = ex2(a);
+    b = ex2(b);
+    if (w != ~0u) {
+      a = (w >> i) & 1 ? a : 0.f;
+      b = (w >> (i + 1)) & 1 ? b : 0.f;
+    }
+    sum = add_f2(sum, pack_f2(a, b));
+    if constexpr (F32) split2(a, b, p[i >> 1], q[i >> 1]);
+    else p[i >> 1] = pack2(BF, a, b);
+  }
 }
 
 // 32 slots from `base` that a tree row sees.
@@ -412,19 +451,16 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
         };
         float mx = -INFINITY;
         if (warp_live) {
+          // the next 32 columns are on their way while these are looked at (f32 has no registers for that)
+          uint32_t x[F32 ? 1 : 2][32];
+          if (!F32) tmem_ld32(S, x[0]);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            uint32_t x[32];
-            tmem_ld32(S + 32 * k, x);
+            uint32_t(&y)[32] = x[F32 ? 0 : k & 1];
+            if (F32) tmem_ld32(S + 32 * k, y);
             tmem_wait_ld();
-            const uint32_t w = word(k);
-            if (w == ~0u) {
-#pragma unroll
-              for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(x[i]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i++) mx = (w >> i) & 1 ? fmaxf(mx, __uint_as_float(x[i])) : mx;
-            }
+            if (!F32 && k < 3) tmem_ld32(S + 32 * (k + 1), x[F32 ? 0 : (k + 1) & 1]);
+            mx = max32(y, word(k), mx);
           }
           if (mx != -INFINITY) mx *= sc;
         }
@@ -454,46 +490,25 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
           l_own = m_own == -INFINITY ? 0.f : l_own * ex2(m_own - m);
           m_own = m;
           const float mm = (m == -INFINITY ? 0.f : m) - SHIFT;
-          float s0 = 0.f, s1 = 0.f;
-          uint32_t held[F32 ? 32 : 1];  // lo parts whose columns hold S yet
+          uint64_t sum = 0;
+          uint32_t x[F32 ? 1 : 2][32];
+          if (!F32) tmem_ld32(S, x[0]);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            uint32_t x[32], p[16], q[F32 ? 16 : 1];
-            tmem_ld32(S + 32 * k, x);
+            uint32_t(&y)[32] = x[F32 ? 0 : k & 1];
+            uint32_t p[16], q[F32 ? 16 : 1];
+            if (F32) tmem_ld32(S + 32 * k, y);
             tmem_wait_ld();
+            if (!F32 && k < 3) tmem_ld32(S + 32 * (k + 1), x[F32 ? 0 : (k + 1) & 1]);
             const uint32_t w = word(k);
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(x[i]), sc, -mm)), p1 = ex2(fmaf(__uint_as_float(x[i + 1]), sc, -mm));
-              if (w != ~0u) {
-                p0 = (w >> i) & 1 ? p0 : 0.f;
-                p1 = (w >> (i + 1)) & 1 ? p1 : 0.f;
-              }
-              s0 += p0;
-              s1 += p1;
-              if constexpr (F32) split2(p0, p1, p[i >> 1], q[i >> 1]);
-              else p[i >> 1] = pack2(BF, p0, p1);
-            }
-            tmem_st16(S + 16 * k, p);  // P over the S columns already read
-            if constexpr (F32) {       // lo parts at 64 + 16 k, once those are read too
-              if (k < 2) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) held[16 * k + i] = q[i];
-              } else {
-                if (k == 2) tmem_st32(S + 64, held);
-                else tmem_st16(S + 112, q);
-                if (k == 2) {
-#pragma unroll
-                  for (int i = 0; i < 16; i++) held[i] = q[i];
-                } else {
-                  uint32_t q2[16];
-#pragma unroll
-                  for (int i = 0; i < 16; i++) q2[i] = held[i];
-                  tmem_st16(S + 96, q2);
-                }
-              }
-            }
+            if (w == ~0u) exp32<F32, BF>(y, ~0u, sc, mm, sum, p, q);
+            else exp32<F32, BF>(y, w, sc, mm, sum, p, q);
+            // P over S columns already read: 16 slots in 8 columns, f32 with 32 slots' lo parts behind their hi parts
+            tmem_st16(S + (F32 ? 32 : 16) * k, p);
+            if constexpr (F32) tmem_st16(S + 32 * k + 16, q);
           }
+          float s0, s1;
+          unpack_f2(sum, s0, s1);
           l_own += s0 + s1;
         }
         tmem_wait_st();
@@ -614,7 +629,7 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
     // ------------------------------------------------------------ MMA issue
     if (lane == 0) {
       constexpr uint32_t I_S = tc_idesc_16(BF, false, 128, 128), I_O = tc_idesc_16(BF, true, 128, HD);
-      const uint32_t q0 = smem_u32(qs), r0 = smem_u32(ring);
+      const uint32_t q_lo = sw128_lo(smem_u32(qs), 16), k_lo = sw128_lo(smem_u32(ring), 16), v_lo = sw128_lo(smem_u32(ring), VK * 128);
       int slot = 0, par = 0, gt = 0;
       auto take = [&]() {
         wait(&c.full[slot], par);
@@ -630,19 +645,19 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
       auto qk = [&](int gi) {
         const uint32_t d = tm + S_COL + 128 * (gi & 1);
         auto block = [&](uint32_t q, bool add) {
+          const uint32_t kk = k_lo + slot * (PIECE >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            tc_mma_ss(d, smem_desc_sw128(q + k * 32, 16, 1024), smem_desc_sw128(r0 + slot * PIECE + k * 32, 16, 1024), I_S,
-                      add || k);
+          for (int k = 0; k < 4; k++) tc_mma_ss_sw128(d, q + k * 2, kk + k * 2, I_S, add || k);
         };
         for (int b = 0; b < NP; b++) {
+          const uint32_t q = q_lo + b * 1024;
           take();
-          block(q0 + b * 16384, b != 0);
-          if (F32) block(q0 + G_::Q_BYTES + b * 16384, true);
+          block(q, b != 0);
+          if (F32) block(q + (G_::Q_BYTES >> 4), true);
           give();
           if (F32) {
             take();
-            block(q0 + b * 16384, true);
+            block(q, true);
             give();
           }
         }
@@ -667,20 +682,23 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
           wait(&c.p_ready[gi & 1], (gi >> 1) & 1);
           tc_fence_after();
           const uint32_t p = tm + S_COL + 128 * (gi & 1);
-          auto block = [&](uint32_t pb, bool add) {
+          auto block = [&](int b, int lo, bool add) {
+            const uint32_t vv = v_lo + slot * (PIECE >> 4);
 #pragma unroll
-            for (int k = 0; k < VK / 16; k++)
-              tc_mma_ts(tm + O_COL, pb + k * 8, smem_desc_sw128(r0 + slot * PIECE + k * 2048, VK * 128, 1024), I_O, add || k);
+            for (int k = 0; k < VK / 16; k++) {
+              const int ks = b * (VK / 16) + k;
+              tc_mma_ts_sw128(tm + O_COL, p + (F32 ? 32 * (ks >> 1) + 8 * (ks & 1) + 16 * lo : 8 * ks), vv + k * 128, I_O,
+                              add || k);
+            }
           };
           for (int b = 0; b < NP; b++) {
-            const uint32_t pb = p + b * (VK / 16) * 8;
             take();
-            block(pb, (j | b) != 0);
-            if (F32) block(pb + 64, true);
+            block(b, 0, (j | b) != 0);
+            if (F32) block(b, 1, true);
             give();
             if (F32) {
               take();
-              block(pb, true);
+              block(b, 0, true);
               give();
             }
           }
@@ -698,18 +716,19 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
     __syncwarp();
   } else if constexpr (TMA) {
     // ------------------------------------------------------------ loads, TMA
-    if (warp == 9 && lane == 0) {
-      int slot = 0, par = 1;  // the first pass over the ring waits for nothing
+    if (lane == 0) {
+      // one tensor copy occupies its thread for a fraction of a microsecond: the pieces go round the warps
+      const int mine = warp - 9;
+      int slot = 0, par = 1, turn = 0;  // the first pass over the ring waits for nothing
       auto put = [&](bool is_v, int z, int b, int hk) {
-        wait(&c.empty[slot], par);
-        mbar_expect_tx(&c.full[slot], PIECE);
-        uint8_t *dst = ring + slot * PIECE;
-        if (!is_v) {
-          tma_3d(dst, &mk, b * 64, hk, z, &c.full[slot]);
-        } else {
-#pragma unroll
-          for (int cb = 0; cb < CB; cb++) tma_3d(dst + cb * VK * 128, &mv, cb * 64, hk, z + b * VK, &c.full[slot]);
+        if (turn == mine) {
+          wait(&c.empty[slot], par);
+          mbar_expect_tx(&c.full[slot], PIECE);
+          uint8_t *dst = ring + slot * PIECE;
+          if (!is_v) tma_4d(dst, &mk, 0, z, b, hk, &c.full[slot]);
+          else tma_4d(dst, &mv, 0, z + b * VK, 0, hk, &c.full[slot]);
         }
+        if (++turn == TMA_WARPS) turn = 0;
         if (++slot == NS) {
           slot = 0;
           par ^= 1;
@@ -734,23 +753,16 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
   } else {
     // ------------------------------------------------------------ loads, one 16-byte unit per thread
     const int lt = tid - 288;
-    // piece `b` of tile `tile`: unit x (of 1024: 8 dims of a slot) -> slot of the tile, unit of the row, place in a piece
-    auto unit = [&](bool is_v, int b, int x, int &key, int &u) -> uint32_t {
-      if (!is_v) {
-        key = x >> 3;
-        u = b * 8 + (x & 7);
-        return key * 128 + (((x & 7) ^ (key & 7)) << 4);
-      }
-      constexpr int UR = HD / 8;  // units of a row
-      const int kr = x / UR;
-      u = x % UR;
-      key = b * VK + kr;
-      return (u >> 3) * (VK * 128) + kr * 128 + (((u & 7) ^ (kr & 7)) << 4);
-    };
-    auto source = [&](bool is_v, uint32_t o, int hk, int u) -> const T * {
-      if constexpr (TREE) return (const T *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + hk) * HD + u * 8;
-      return (const T *)(is_v ? a.v : a.k) + (int64_t)o * (is_v ? a.vrow : a.krow) + hk * (is_v ? a.vhead : a.khead) + u * 8;
-    };
+    // A thread copies 16-byte units (8 dims) of the rows lt/8, lt/8 + LD/8, ...  of a tile, K and V alike, so its row
+    // pointers are made once per tile: K piece b takes the block b of all of its rows, V piece b every block of the
+    // rows that lie in it.
+    constexpr int RSTEP = LD / 8, NR = TC_KEYS / RSTEP, RV = VK / RSTEP;
+    const int r0 = lt >> 3, u0 = lt & 7, swz = r0 * 128 + ((u0 ^ (r0 & 7)) << 4);
+    // unit i (of NR) of a piece: its row and its block, and its place in the piece
+    auto unit_row = [&](bool is_v, int b, int i) { return is_v ? b * RV + i % RV : i; };
+    auto unit_block = [&](bool is_v, int b, int i) { return is_v ? i / RV : b; };
+    auto unit_at = [&](bool is_v, int i) { return swz + (is_v ? (i / RV) * (VK * 128) + (i % RV) * (RSTEP * 128) : i * (RSTEP * 128)); };
+    const T *row_p[NR];  // nullptr: no such slot
     constexpr uint32_t NONE = 0xffffffffu;
     // pool rows (or prompt rows) of a tile's slots
     auto offsets = [&](const Seg &g, int tile) {
@@ -776,6 +788,16 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
       }
       named_bar(4, LD);
     };
+    auto rows_of = [&](bool is_v, int tile, int hk) {
+#pragma unroll
+      for (int i = 0; i < NR; i++) {
+        const uint32_t o = c.rowoff[tile & 1][r0 + i * RSTEP];
+        const T *p;
+        if constexpr (TREE) p = (const T *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + hk) * HD;
+        else p = (const T *)(is_v ? a.v : a.k) + (int64_t)o * (is_v ? a.vrow : a.krow) + hk * (is_v ? a.vhead : a.khead);
+        row_p[i] = o == NONE ? nullptr : p + u0 * 8;
+      }
+    };
     // the pieces in the order of their use: K(t0), then K(j), V(j - 1), then V(t1 - 1)
     Seg g;
     int si = -1, pj = 0, pb = 0;
@@ -798,7 +820,10 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
         is_v = false;
         more = true;
       }
-      if (!is_v && pb == 0) offsets(g, pj);
+      if (pb == 0) {
+        if (!is_v) offsets(g, pj);
+        rows_of(is_v, is_v ? pj - 1 : pj, g.hk);
+      }
       return true;
     };
     int slot = 0, par = 1;  // the first pass over the ring waits for nothing
@@ -809,91 +834,81 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
       }
     };
     if constexpr (F32) {
-      // registers hold the next piece while this one is split and stored
-      struct Piece {
-        float x[4][8];
-        bool v, first;
-        int b, si;
-      };
-      auto fetch = [&](Piece &p) {
-        p.v = is_v;
-        p.b = pb;
-        p.si = si;
-        const int tile = is_v ? pj - 1 : pj;
-        p.first = tile == g.t0 && pb == 0;
-        const bool vec = TREE || a.vec;
+      // a thread's four units of a piece are in registers: each is loaded for the next piece as soon as it is
+      // split and stored for this one
+      float x[4][8];
+      const bool vec = TREE || a.vec;
+      // fixed i: the row of a unit depends on the piece only through b, which a switch over few values resolves
+      auto load = [&](int i) {
+        const float *src = nullptr;
+        if (!is_v) {
+          src = (const float *)row_p[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          int key, u;
-          unit(is_v, pb, lt + 256 * i, key, u);
-          const uint32_t o = c.rowoff[tile & 1][key];
-          if (o == NONE) {
+          for (int r = 0; r < NR; r++)
+            if (r == unit_row(true, pb, i)) src = (const float *)row_p[r];
+        }
+        if (!src) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) p.x[i][k] = 0.f;
+          for (int k = 0; k < 8; k++) x[i][k] = 0.f;
+        } else {
+          src += unit_block(is_v, pb, i) * 64;
+          if (vec) {
+            *(float4 *)x[i] = *(const float4 *)src;
+            *(float4 *)(x[i] + 4) = *(const float4 *)(src + 4);
           } else {
-            const float *src = (const float *)source(is_v, o, g.hk, u);
-            if (vec) {
-              *(float4 *)p.x[i] = *(const float4 *)src;
-              *(float4 *)(p.x[i] + 4) = *(const float4 *)(src + 4);
-            } else {
 #pragma unroll
-              for (int k = 0; k < 8; k++) p.x[i][k] = src[k];
-            }
+            for (int k = 0; k < 8; k++) x[i][k] = src[k];
           }
         }
       };
       float fk = 1.f, fv = 1.f;
-      int es = 0;
-      auto store = [&](const Piece &p) {
-        if (p.first) {
+      bool have = advance();
+      if (have) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) load(i);
+      }
+      while (have) {
+        const bool v = is_v, first = (v ? pj - 1 : pj) == g.t0 && pb == 0;
+        const int wi = si & 7;
+        have = advance();
+        int e = 0;
+        if (first) {
           float mx = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(p.x[i][k]));
+            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[i][k]));
           mx = warp_max(mx);
           named_bar(4, LD);
           if (lane == 0) c.amax[warp - 9] = mx;
           named_bar(4, LD);
 #pragma unroll
           for (int i = 0; i < 8; i++) mx = fmaxf(mx, c.amax[i]);
-          const int e = scale_exp(mx);
-          (p.v ? fv : fk) = exp2_int(e);
-          es = e;
+          e = scale_exp(mx);
+          (v ? fv : fk) = exp2_int(e);
         }
-        const float f = p.v ? fv : fk;
+        const float f = v ? fv : fk;
         const int s_hi = slot;
         wait(&c.empty[slot], par);
         step();
         const int s_lo = slot;
         wait(&c.empty[slot], par);
         step();
-        if (p.first && lt == 0) (p.v ? c.ve : c.ke)[p.si & 7] = es;
+        if (first && lt == 0) (v ? c.ve : c.ke)[wi] = e;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          int key, u;
-          const uint32_t at = unit(p.v, p.b, lt + 256 * i, key, u);
+          const uint32_t at = unit_at(v, i);
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) split2(p.x[i][2 * k] * f, p.x[i][2 * k + 1] * f, hi[k], lo[k]);
+          for (int k = 0; k < 4; k++) split2(x[i][2 * k] * f, x[i][2 * k + 1] * f, hi[k], lo[k]);
           *(uint4 *)(ring + s_hi * PIECE + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4 *)(ring + s_lo * PIECE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (have) load(i);
         }
         fence_proxy_async_smem();
         mbar_arrive(&c.full[s_hi]);
         mbar_arrive(&c.full[s_lo]);
-      };
-      Piece A, B;
-      bool have = advance();
-      if (have) fetch(A);
-      while (have) {
-        have = advance();
-        if (have) fetch(B);
-        store(A);
-        if (!have) break;
-        have = advance();
-        if (have) fetch(A);
-        store(B);
       }
     } else {
       constexpr int D = 5;  // pieces in flight per thread
@@ -907,25 +922,35 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
       while (advance()) {
         wait(&c.empty[slot], par);
         const uint32_t base = smem_u32(ring + slot * PIECE);
-        const uint32_t *off = c.rowoff[(is_v ? pj - 1 : pj) & 1];
+        auto piece = [&](auto v_const, auto b_const) {  // both known: row_p stays in registers
+          constexpr bool V = decltype(v_const)::value;
+          constexpr int B = decltype(b_const)::value;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          int key, u;
-          const uint32_t dst = base + unit(is_v, pb, lt + 128 * i, key, u);
-          const uint32_t o = off[key];
-          const bool ok = o != NONE;
-          const T *src = source(is_v, ok ? o : 0, g.hk, u);
-          if (TREE || a.vec) {
-            cp_async16(dst, src, ok);
-          } else {
-            T e[8];
+          for (int i = 0; i < NR; i++) {
+            const T *src = row_p[unit_row(V, B, i)];
+            const bool ok = src != nullptr;
+            src = ok ? src + unit_block(V, B, i) * 64 : (const T *)(TREE ? a.kv.k : a.k);
+            const uint32_t dst = base + unit_at(V, i);
+            if (TREE || a.vec) {
+              cp_async16(dst, src, ok);
+            } else {
+              T e[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) e[k] = ok ? src[k] : from_f<T>(0.f);
-            const uint4 w = *(uint4 *)e;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                         : "memory");
+              for (int k = 0; k < 8; k++) e[k] = ok ? src[k] : from_f<T>(0.f);
+              const uint4 w = *(uint4 *)e;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                           : "memory");
+            }
           }
-        }
+        };
+        auto of_kind = [&](auto v_const) {
+          if (NP == 1 || pb == 0) piece(v_const, std::integral_constant<int, 0>());
+          else if (NP == 2 || pb == 1) piece(v_const, std::integral_constant<int, NP >= 2 ? 1 : 0>());
+          else if (pb == 2) piece(v_const, std::integral_constant<int, NP >= 4 ? 2 : 0>());
+          else piece(v_const, std::integral_constant<int, NP >= 4 ? 3 : 0>());
+        };
+        if (is_v) of_kind(std::true_type());
+        else of_kind(std::false_type());
         cp_async_commit();
         issued++;
         step();
@@ -1031,16 +1056,16 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled g_encode = nullptr;
 
-// Rows [n_rows][nkv] of hd dims in boxes of 64 dims x box_rows rows.
+// Rows [n_rows][nkv] of hd dims as [head][64-dim block][row][64], in boxes of box_rows rows x box_blocks blocks.
 bool make_map(CUtensorMap *m, bool bf16, const void *p, int64_t row, int64_t head, int hd, int nkv, int n_rows,
-              int box_rows) {
+              int box_rows, int box_blocks) {
   if (nkv == 1) head = hd;  // never used; must be a stride all the same
   const int64_t lim = (int64_t)1 << 39;
   if (!g_encode || (uintptr_t)p % 16 || row < 8 || head < 8 || row % 8 || head % 8 || row > lim || head > lim) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nkv, (cuuint64_t)n_rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
-  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, one[3] = {1, 1, 1};
-  return g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(p),
+  const cuuint64_t dims[4] = {64, (cuuint64_t)n_rows, (cuuint64_t)hd / 64, (cuuint64_t)nkv};
+  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, 128, (cuuint64_t)head * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1}, one[4] = {1, 1, 1, 1};
+  return g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p),
                   dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1066,8 +1091,8 @@ cudaError_t prompt_hd(AttnOp a, cudaStream_t st) {
   const dim3 grid((unsigned)(tiles * a.nh));
   using G = Geo<TY, HD>;
   if constexpr (TY != TY_F32) {
-    if (make_map(&mk, TY == TY_BF16, a.k, a.krow, a.khead, HD, a.nkv, a.n_rows, TC_KEYS) &&
-        make_map(&mv, TY == TY_BF16, a.v, a.vrow, a.vhead, HD, a.nkv, a.n_rows, G::VK))
+    if (make_map(&mk, TY == TY_BF16, a.k, a.krow, a.khead, HD, a.nkv, a.n_rows, TC_KEYS, 1) &&
+        make_map(&mv, TY == TY_BF16, a.v, a.vrow, a.vhead, HD, a.nkv, a.n_rows, G::VK, G::CB))
       return launch_pdl(attn_tc_kernel<TY, HD, false, true>, grid, G::threads(true), G::SMEM, st, a, mk, mv);
   }
   memset(&mk, 0, sizeof mk);

@@ -71,11 +71,11 @@ CW_DEV void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar) 
 
 // Tile of a tensor map (global -> shared through the TMA engine), completes on
 // an mbarrier.  x * element size a multiple of 16 bytes, dst 1024-byte aligned.
-CW_DEV void tma_3d(void *dst, const void *map, int x, int y, int z, uint64_t *bar) {
+CW_DEV void tma_4d(void *dst, const void *map, int x, int y, int z, int w, uint64_t *bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-      "[%5];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
 // 16-byte asynchronous copy by this thread, or 16 zero bytes when !valid.
@@ -183,21 +183,34 @@ constexpr uint32_t tc_idesc_f16(int M, int N) {
 // K-major: rows are M or N, the next 8 rows `sbo` bytes on, the next 16 K
 // elements of the 64 in a row 32 bytes on; lbo is not used.  MN-major: rows are
 // K, the next 8 of them `sbo` bytes on, the next 64 M or N elements `lbo`.
-CW_DEV uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return smem_desc_kmajor(saddr, lbo, sbo) | (2ull << 61);
-}
+// Its low and its high word.  One thread issues every MMA of
+// a tile, so what it computes per MMA counts: the high word is a constant and
+// an address step is one addition to the low word.
+CW_DEV constexpr uint32_t sw128_lo(uint32_t saddr, uint32_t lbo) { return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
+constexpr uint32_t SW128_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // sbo 1024, version 1, layout 2
 // Instruction descriptor of kind::f16 with A and B of one type (f16, or bf16:
 // formats 1 at [7,10) and [10,13)), B MN-major with b_mn (bit 16).
 constexpr uint32_t tc_idesc_16(bool bf16, bool b_mn, int M, int N) {
   return tc_idesc_f16(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
-// D[tmem] (+)= A[smem desc] * B[smem desc], issued by one thread.
-CW_DEV void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem] for low descriptor words, issued by one thread.
+CW_DEV void tc_mma_ss_sw128(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "n"(SW128_HI)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem] for a low descriptor word, issued by one thread.
+CW_DEV void tc_mma_ts_sw128(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "n"(SW128_HI)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem desc], issued by one thread.  accumulate = 0
@@ -215,6 +228,23 @@ CW_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_
 CW_DEV void tc_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
+}
+// Two fp32 operations in one instruction.
+CW_DEV uint64_t pack_f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+CW_DEV void unpack_f2(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+CW_DEV uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+CW_DEV uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 // Make generic-proxy shared-memory writes visible to the async proxy (the
 // tensor cores read B operands through it).

@@ -12,10 +12,13 @@
 //
 // Roles: warps 0-3 and 4-7 take the softmax of alternate tiles, one row per
 // thread; warp 8 issues the MMAs (two S tiles in flight, so the tensor cores
-// work on one while the other's softmax runs); warp 9 (prompt: TMA tensor maps)
-// or warps 9-12 (tree, and prompts whose rows TMA cannot address) fill a ring of
+// work on one while the other's softmax runs); the warps from 9 on fill a ring of
 // 16 KB pieces in the order in which the MMAs use them: K as 128 slots x 64
-// dims, V as 8192/HD slots x HD dims, both with 128-byte swizzle.
+// dims, V as 8192/HD slots x HD dims in groups of 16 slots, both with 128-byte
+// swizzle.  f16 and bf16 pieces go round four warps, each lane one tensor copy
+// (TMA boxes of whole pages: K as many slots as a page holds in a power of two, V
+// 16); pages that are no multiple of 16 slots and rows that TMA cannot address are
+// copied 16 bytes a lane (or by element).
 //
 // f32 rows are split in two f16 parts, x 2^e = hi + lo to 2^-22 of x, and every
 // product is hi hi + lo hi + hi lo (lo lo is below 2^-22 of it): three f16 MMAs
@@ -40,7 +43,7 @@ namespace cw {
 namespace {
 
 constexpr int PIECE = 16384;
-constexpr int TMA_WARPS = 3;
+constexpr int LOAD_WARPS = 4;  // f16, bf16
 constexpr float P_SHIFT_F16 = 7.f;  // p <= 2^(8+7) < 65504
 constexpr float RESCALE_AT = 8.f;
 
@@ -59,25 +62,29 @@ struct Geo {
   static constexpr int VK = 8192 / HD;       // slots of a V piece
   static constexpr int NS = F32 ? (HD == 256 ? 5 : HD == 128 ? 9 : 11) : (HD == 256 ? 9 : HD == 128 ? 11 : 12);
   static constexpr int SMEM = Q_BYTES * (F32 ? 2 : 1) + NS * PIECE + 1024;
-  static constexpr int LOADERS = F32 ? 256 : 128;
-  static constexpr int threads(bool tma) { return 288 + (tma ? 32 * TMA_WARPS : LOADERS); }
+  static constexpr int LOADERS = F32 ? 256 : 32 * LOAD_WARPS, THREADS = 288 + LOADERS;
+  static constexpr int VG = CB * 2048;       // 16 slots of a V piece: [block][16 slots][128 B]
 };
-constexpr int WIN = 4;  // f32: tiles of a window
+constexpr int WIN = 8;  // f32: tiles of a window
+constexpr int SEG_COST = 4;  // tree: what a segment's start and end cost, in tiles
 
 struct Ctl {
-  uint64_t full[12], empty[12], s_full[2], p_ready[2], pv_done, q_full, o_free, o_done, drained;
+  uint64_t full[12], empty[12], s_full[2], p_ready[2], pv_done, q_full, o_free, o_done, drained, tail[LOAD_WARPS];
   int64_t u0, u1;
+  int hk0, mt0, t00;
   uint32_t tmem;
   volatile int abort, bad;
   int s0, tile0, begin, end;
-  int64_t rem;
   unsigned badrows[4];
   float mref[TC_ROWS];
   float2 ml[2][TC_ROWS];
-  uint32_t rowoff[2][TC_KEYS];
+  uint32_t rowoff[4][TC_KEYS];  // f32, [tile mod 4]: rows of the slots
   // f32: exponents that Q rows, and a window's K and V, were multiplied by (the loaders run up to three windows ahead)
   int qe[TC_ROWS], ke[8], ve[8];
   float amax[8];
+};
+struct CtlF32 : Ctl {
+  alignas(16) uint8_t stage[8][1024];
 };
 
 // Where one segment of work lies: the tiles [w0, w1) of a row tile's nt, and
@@ -88,10 +95,12 @@ struct Seg {
 };
 
 CW_HOST_DEV int tree_tiles(int n) { return (n + TC_KEYS - 1) / TC_KEYS; }
+// Units of a segment: first SEG_COST that stand for its fixed cost, then its tiles.
+CW_HOST_DEV int seg_units(int n) { return tree_tiles(n) + SEG_COST; }
 CW_DEV int64_t seq_units(const AttnOp &a, int s) {
   const TreeSeq q = tree_seq(a, s);
   const int G = a.nh / a.nkv;
-  return q.live ? (int64_t)a.nkv * ((q.live * G + TC_ROWS - 1) / TC_ROWS) * tree_tiles(q.n) : 0;
+  return q.live ? (int64_t)a.nkv * ((q.live * G + TC_ROWS - 1) / TC_ROWS) * seg_units(q.n) : 0;
 }
 CW_DEV int64_t warp_scan(int64_t v) {  // inclusive
   const int lane = threadIdx.x & 31;
@@ -109,15 +118,17 @@ struct TreeWalk {
   int64_t left;
   CW_DEV void start(const AttnOp &a, const Ctl &c) {
     s = c.s0;
+    hk = c.hk0;
+    mt = c.mt0;
+    t0 = c.t00;
     left = c.u1 - c.u0;
-    const TreeSeq q = tree_seq(a, s);
-    const int G = a.nh / a.nkv, nt = tree_tiles(q.n), mts = (q.live * G + TC_ROWS - 1) / TC_ROWS;
-    const int64_t i = c.rem / nt;
-    t0 = (int)(c.rem - i * nt);
-    mt = (int)(i % mts);
-    hk = (int)(i / mts);
   }
   CW_DEV bool next(const AttnOp &a, Seg &g) {
+    while (step(a, g))
+      if (g.t1 > g.t0) return true;  // units without tiles: another CTA's segment
+    return false;
+  }
+  CW_DEV bool step(const AttnOp &a, Seg &g) {
     if (left <= 0) return false;
     const int G = a.nh / a.nkv;
     g.ts = tree_seq(a, s);
@@ -126,11 +137,12 @@ struct TreeWalk {
     g.s = s;
     g.hk = hk;
     g.mt = mt;
-    g.t0 = t0;
-    g.t1 = (int)min((int64_t)g.nt, t0 + left);
-    left -= g.t1 - g.t0;
+    const int end = (int)min((int64_t)seg_units(g.ts.n), t0 + left);  // units [t0, end) of the segment
+    g.t0 = max(t0 - SEG_COST, 0);
+    g.t1 = max(end - SEG_COST, 0);
+    left -= end - t0;
     t0 = 0;
-    if (g.t1 == g.nt && ++mt * TC_ROWS >= g.ts.live * G) {
+    if (end == seg_units(g.ts.n) && ++mt * TC_ROWS >= g.ts.live * G) {
       mt = 0;
       if (++hk == a.nkv) {
         hk = 0;
@@ -202,6 +214,61 @@ CW_DEV void exp32(const uint32_t (&x)[32], uint32_t w, float sc, float mm, uint6
   }
 }
 
+// 32 rows of a warp, one per lane in registers, to their places in global memory: through shared memory, so that
+// UNITS neighbouring lanes write 16-byte units of one row (32 different rows at once would cost 32 passes of the
+// load/store unit).  stage: 32 x UNITS x 16 bytes of the warp.  dst: the lane's row; ok: whether it is there.
+template <int UNITS, class E>
+CW_DEV void flush_rows(uint8_t *stage, const uint32_t *x, E *dst, bool ok, bool vec) {
+  constexpr int M = UNITS - 1, SH = UNITS == 4 ? 1 : 2, N = 16 / (int)sizeof(E);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < UNITS; u++)
+    *(uint4 *)(stage + (lane * UNITS + (u ^ ((lane >> SH) & M))) * 16) = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < UNITS; i++) {
+    const int r = (i * 32 + lane) / UNITS, u = lane & M;
+    const uint4 w = *(const uint4 *)(stage + (r * UNITS + (u ^ ((r >> SH) & M))) * 16);
+    E *d = (E *)__shfl_sync(0xffffffffu, (unsigned long long)dst, r) + u * N;
+    if (!__shfl_sync(0xffffffffu, (int)ok, r)) continue;
+    if (vec) {
+      *(uint4 *)d = w;
+    } else {
+      const E *e = (const E *)&w;
+#pragma unroll
+      for (int k = 0; k < N; k++) d[k] = e[k];
+    }
+  }
+  __syncwarp();
+}
+// The way back.
+template <int UNITS>
+CW_DEV void fetch_rows(uint8_t *stage, uint32_t *x, const float *src, bool ok, bool vec) {
+  constexpr int M = UNITS - 1, SH = UNITS == 4 ? 1 : 2;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < UNITS; i++) {
+    const int r = (i * 32 + lane) / UNITS, u = lane & M;
+    const float *p = (const float *)__shfl_sync(0xffffffffu, (unsigned long long)src, r) + u * 4;
+    float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (__shfl_sync(0xffffffffu, (int)ok, r)) {
+      if (vec) w = *(const float4 *)p;
+      else w = make_float4(p[0], p[1], p[2], p[3]);
+    }
+    *(float4 *)(stage + (r * UNITS + (u ^ ((r >> SH) & M))) * 16) = w;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < UNITS; u++) {
+    const uint4 w = *(const uint4 *)(stage + (lane * UNITS + (u ^ ((lane >> SH) & M))) * 16);
+    x[4 * u] = w.x;
+    x[4 * u + 1] = w.y;
+    x[4 * u + 2] = w.z;
+    x[4 * u + 3] = w.w;
+  }
+  __syncwarp();
+}
+
 // 32 slots from `base` that a tree row sees.
 CW_DEV uint32_t tree_word(const TreeSeq &q, uint64_t bits, int base) {
   const int d = q.len - base;  // committed slots of the word
@@ -214,27 +281,28 @@ CW_DEV uint32_t tree_word(const TreeSeq &q, uint64_t bits, int base) {
 
 }  // namespace
 
-template <int TY, int HD, bool TREE, bool TMA>
-__global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
+// kbox: slots of a K box, 0 where tensor copies are not used.
+template <int TY, int HD, bool TREE>
+__global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
     attn_tc_kernel(const __grid_constant__ AttnOp a, const __grid_constant__ CUtensorMap mk,
-                   const __grid_constant__ CUtensorMap mv) {
+                   const __grid_constant__ CUtensorMap mv, int kbox) {
   using G_ = Geo<TY, HD>;
   using T = typename TypeOf<TY>::T;
   constexpr bool F32 = TY == TY_F32, BF = TY == TY_BF16;
   constexpr int LD = G_::LOADERS;
   constexpr int CB = G_::CB, NP = G_::NP, VK = G_::VK, NS = G_::NS;
   constexpr int O_COL = 0, S_COL = 256;
-  __shared__ Ctl c;
+  __shared__ typename std::conditional<F32, CtlF32, Ctl>::type c;
   extern __shared__ uint8_t dyn[];
   uint8_t *qs = (uint8_t *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
   uint8_t *ring = qs + G_::Q_BYTES * (F32 ? 2 : 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.nh / a.nkv;
 
-  pdl_trigger();
+  if (warp == 8) tmem_alloc(&c.tmem, 512);
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
-      mbar_init(&c.full[i], TMA ? 1 : LD);
+      mbar_init(&c.full[i], F32 ? LD : 1);
       mbar_init(&c.empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -246,12 +314,14 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
     mbar_init(&c.o_free, 256);
     mbar_init(&c.o_done, 1);
     mbar_init(&c.drained, 1);
+    for (int i = 0; i < LOAD_WARPS; i++) mbar_init(&c.tail[i], 1);
     mbar_fence_init();
     c.abort = 0;
     c.bad = 0;
   }
   if (tid < 4) c.badrows[tid] = 0;
   pdl_wait();
+  pdl_trigger();  // after the wait: the joining kernel may read the lengths before its own wait
   if (warp == 0) {  // this CTA's work
     const int ch = (a.n_seq + 31) / 32, i0 = min(a.n_seq, lane * ch), i1 = min(a.n_seq, i0 + ch);
     int64_t mine = 0;
@@ -290,23 +360,32 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
         }
         if (u0 < at + n) {
           c.s0 = i;
-          c.rem = u0 - at;
           c.begin = b;
           c.end = e;
           c.tile0 = (int)(u0 - at);
+          if constexpr (TREE) {
+            const TreeSeq q = tree_seq(a, i);
+            const int64_t rem = u0 - at;
+            const int nt = seg_units(q.n), mts = (q.live * G + TC_ROWS - 1) / TC_ROWS;
+            const int64_t x = rem <= 0x7fffffff ? (uint32_t)rem / (uint32_t)nt : rem / nt;
+            c.t00 = (int)(rem - x * nt);
+            c.mt0 = (int)x % mts;  // x < n_kv mts
+            c.hk0 = (int)x / mts;
+          }
           break;
         }
         at += n;
       }
     }
   }
-  __syncthreads();
-  if (c.u0 >= c.u1) return;
-  if (warp == 0) tmem_alloc(&c.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = c.tmem;
+  if (c.u0 >= c.u1) {
+    if (warp == 8) tmem_dealloc(tm, 512);
+    return;
+  }
 
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     if (!mbar_wait(bar, parity, &c.abort)) {
@@ -552,6 +631,9 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
           }
         }
       }
+      // Q is read no more (f32: it is, by the next window)
+      uint8_t *stage = qs + warp * 2048;
+      if constexpr (F32) stage = c.stage[warp];
       if (warp_live) {
 #pragma unroll 1
         for (int k = 0; k < HD / 64; k++) {
@@ -559,29 +641,23 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
           uint32_t x[32];
           tmem_ld32(tm + lane_base + O_COL + col, x);
           tmem_wait_ld();
-          if (!have) continue;
-          T *o = (T *)a.o + row * a.orow + h * a.ohead + col;
+          T *o = (T *)a.o + (have ? row * a.orow + h * a.ohead : 0) + col;
           if constexpr (F32) {
             float *dst = part ? part + col : (float *)o;
             const bool v4 = part || ovec;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float old[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
-              if (!first) {
-                if (v4) *(float4 *)old = *(const float4 *)(dst + i);
-                else
-                  for (int d = 0; d < 4; d++) old[d] = dst[i + d];
-              }
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t old[8];
+              float f[8];
+              if (!first) fetch_rows<2>(stage, old, dst + i, have, v4);
 #pragma unroll
-              for (int d = 0; d < 4; d++) {
+              for (int d = 0; d < 8; d++) {
                 f[d] = __uint_as_float(x[i + d]) * f_new;
-                if (!first) f[d] = fmaf(old[d], f_old, f[d]);
+                if (!first) f[d] = fmaf(__uint_as_float(old[d]), f_old, f[d]);
                 f[d] = l == 0.f ? 0.f : f[d] * inv;
                 bad |= !(fabsf(f[d]) < INFINITY);
               }
-              if (v4) *(float4 *)(dst + i) = *(const float4 *)f;
-              else
-                for (int d = 0; d < 4; d++) dst[i + d] = f[d];
+              flush_rows<2>(stage, (const uint32_t *)f, dst + i, have, v4);
             }
           } else {
             float f[32];
@@ -592,16 +668,12 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
             }
             if (TREE && part) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *(float4 *)(part + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-            } else if (ovec) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 8)
-                *(uint4 *)(o + i) = make_uint4(pack2(BF, f[i], f[i + 1]), pack2(BF, f[i + 2], f[i + 3]),
-                                               pack2(BF, f[i + 4], f[i + 5]), pack2(BF, f[i + 6], f[i + 7]));
+              for (int i = 0; i < 32; i += 16) flush_rows<4>(stage, (const uint32_t *)f + i, part + col + i, have, true);
             } else {
+              uint32_t w[16];
 #pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = from_f<T>(f[i]);
+              for (int i = 0; i < 16; i++) w[i] = pack2(BF, f[2 * i], f[2 * i + 1]);
+              flush_rows<4>(stage, w, o, have, ovec);
             }
           }
         }
@@ -629,7 +701,7 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
     // ------------------------------------------------------------ MMA issue
     if (lane == 0) {
       constexpr uint32_t I_S = tc_idesc_16(BF, false, 128, 128), I_O = tc_idesc_16(BF, true, 128, HD);
-      const uint32_t q_lo = sw128_lo(smem_u32(qs), 16), k_lo = sw128_lo(smem_u32(ring), 16), v_lo = sw128_lo(smem_u32(ring), VK * 128);
+      const uint32_t q_lo = sw128_lo(smem_u32(qs), 16), k_lo = sw128_lo(smem_u32(ring), 16), v_lo = sw128_lo(smem_u32(ring), 2048);
       int slot = 0, par = 0, gt = 0;
       auto take = [&]() {
         wait(&c.full[slot], par);
@@ -687,7 +759,7 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
 #pragma unroll
             for (int k = 0; k < VK / 16; k++) {
               const int ks = b * (VK / 16) + k;
-              tc_mma_ts_sw128(tm + O_COL, p + (F32 ? 32 * (ks >> 1) + 8 * (ks & 1) + 16 * lo : 8 * ks), vv + k * 128, I_O,
+              tc_mma_ts_sw128(tm + O_COL, p + (F32 ? 32 * (ks >> 1) + 8 * (ks & 1) + 16 * lo : 8 * ks), vv + k * (G_::VG >> 4), I_O,
                               add || k);
             }
           };
@@ -714,145 +786,246 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
       mbar_wait(&c.drained, 0, &no);
     }
     __syncwarp();
-  } else if constexpr (TMA) {
-    // ------------------------------------------------------------ loads, TMA
-    if (lane == 0) {
-      // one tensor copy occupies its thread for a fraction of a microsecond: the pieces go round the warps
-      const int mine = warp - 9;
-      int slot = 0, par = 1, turn = 0;  // the first pass over the ring waits for nothing
-      auto put = [&](bool is_v, int z, int b, int hk) {
-        if (turn == mine) {
-          wait(&c.empty[slot], par);
-          mbar_expect_tx(&c.full[slot], PIECE);
-          uint8_t *dst = ring + slot * PIECE;
-          if (!is_v) tma_4d(dst, &mk, 0, z, b, hk, &c.full[slot]);
-          else tma_4d(dst, &mv, 0, z + b * VK, 0, hk, &c.full[slot]);
+  } else if constexpr (!F32) {
+    // ------------------------------------------------------------ loads, a piece per warp
+    const int mine = warp - 9;
+    int slot = 0, par = 1, turn = 0, tails = 0;  // the first pass over the ring waits for nothing
+    // pool row (or prompt row) of a slot, -1: none
+    auto row_of = [&](const Seg &g, int sl) -> int64_t {
+      if constexpr (TREE) {
+        if (sl >= g.ts.n) return -1;
+        const int64_t r = cwp_row(a.kv.table + (int64_t)g.s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, sl);
+        if (r < 0) {
+          c.bad = 1;
+          atomicOr(a.err, OPE_PAGE);
         }
-        if (++turn == TMA_WARPS) turn = 0;
-        if (++slot == NS) {
-          slot = 0;
-          par ^= 1;
-        }
-      };
-      Seg g;
-      while (next(g)) {
-        for (int j = 0; j <= g.nt; j++) {
-          if (j < g.nt)
-            for (int b = 0; b < NP; b++) put(false, pbegin + j * TC_KEYS, b, g.hk);
-          if (j > 0)
-            for (int b = 0; b < NP; b++) put(true, pbegin + (j - 1) * TC_KEYS, b, g.hk);
-        }
+        return r;
+      } else {
+        return pbegin + sl < pend ? pbegin + sl : -1;
       }
-      if (c.abort) {  // copies may still be landing: a millisecond is far beyond any of them
-        const long long t0 = cycles_now();
-        while (cycles_now() - t0 < 2000000ll) {
-        }
-      }
-    }
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------ loads, one 16-byte unit per thread
-    const int lt = tid - 288;
-    // A thread copies 16-byte units (8 dims) of the rows lt/8, lt/8 + LD/8, ...  of a tile, K and V alike, so its row
-    // pointers are made once per tile: K piece b takes the block b of all of its rows, V piece b every block of the
-    // rows that lie in it.
-    constexpr int RSTEP = LD / 8, NR = TC_KEYS / RSTEP, RV = VK / RSTEP;
-    const int r0 = lt >> 3, u0 = lt & 7, swz = r0 * 128 + ((u0 ^ (r0 & 7)) << 4);
-    // unit i (of NR) of a piece: its row and its block, and its place in the piece
-    auto unit_row = [&](bool is_v, int b, int i) { return is_v ? b * RV + i % RV : i; };
-    auto unit_block = [&](bool is_v, int b, int i) { return is_v ? i / RV : b; };
-    auto unit_at = [&](bool is_v, int i) { return swz + (is_v ? (i / RV) * (VK * 128) + (i % RV) * (RSTEP * 128) : i * (RSTEP * 128)); };
-    const T *row_p[NR];  // nullptr: no such slot
-    constexpr uint32_t NONE = 0xffffffffu;
-    // pool rows (or prompt rows) of a tile's slots
-    auto offsets = [&](const Seg &g, int tile) {
-      named_bar(4, LD);  // the readers of two tiles ago are through
-      const int sl = tile * TC_KEYS + lt;
-      if (lt < TC_KEYS) {
-        uint32_t o = NONE;
-        if constexpr (TREE) {
-          if (sl < g.ts.n) {
-            const int64_t x = cwp_row(a.kv.table + (int64_t)g.s * a.kv.stride, a.kv.stride, a.kv.n_pages, a.kv.page_size, sl);
-            if (x >= 0) {
-              o = (uint32_t)x;
+    };
+    auto put = [&](const Seg &g, bool is_v, int tile, int b) {
+      if (turn == mine) {
+        wait(&c.empty[slot], par);
+        uint8_t *dst = ring + slot * PIECE;
+        const int n = TREE ? g.ts.n : pend - pbegin, sl0 = tile * TC_KEYS + (is_v ? b * VK : 0);
+        if (kbox) {
+          // a tile that ends inside: boxes with a slot at least, then zeros over the V rows behind the last slot
+          // (whatever they hold meets zero weights, which must not make NaN); K there meets the mask
+          const int step = is_v ? 16 : kbox, have = min(n - sl0, is_v ? VK : TC_KEYS);  // slots of the piece
+          const int boxes = have <= 0 ? 0 : (have + step - 1) / step;
+          const bool tail = is_v && have < VK;
+          uint64_t *bar = tail ? &c.tail[mine] : &c.full[slot];
+          if (lane == 0 && boxes) mbar_expect_tx(bar, boxes * (is_v ? G_::VG : step * 128));
+          __syncwarp();
+          if (lane < boxes) {
+            int64_t r = row_of(g, sl0 + lane * step);
+            if (r < 0) r = 0;  // a bad page: any rows do, exact_row comes after
+            if (!is_v) tma_4d(dst + lane * step * 128, &mk, 0, (int)r, b, g.hk, bar);
+            else tma_4d(dst + lane * G_::VG, &mv, 0, (int)r, 0, g.hk, bar);
+          }
+          if (tail) {
+            if (boxes) {
+              wait(bar, tails & 1);
+              tails++;
+            }
+            constexpr int UR = HD / 8;
+            for (int i = max(have, 0) * UR + lane; i < VK * UR; i += 32) {
+              const int key = i / UR, u = i % UR;
+              *(uint4 *)(dst + (key >> 4) * G_::VG + (u >> 3) * 2048 + (key & 15) * 128 + ((u & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.full[slot]);
+          }
+        } else {
+          constexpr int KL = TC_KEYS / 32, VL = VK / 32, UR = HD / 8, VR = 32 / UR;  // rows a lane looks up; V: units of a row, rows a step
+          const T *base = (const T *)(TREE ? (is_v ? a.kv.v : a.kv.k) : (is_v ? a.v : a.k));
+          const int64_t rs = TREE ? (int64_t)a.nkv * HD : is_v ? a.vrow : a.krow, hs = TREE ? HD : is_v ? a.vhead : a.khead;
+          base += g.hk * hs;
+          int64_t off[KL];
+#pragma unroll
+          for (int i = 0; i < KL; i++) {
+            off[i] = -1;
+            if (i < VL || !is_v) off[i] = row_of(g, sl0 + lane + 32 * i);
+          }
+#pragma unroll 1
+          for (int i8 = 0; i8 < 4; i8++) {  // 8 units a lane at a time: the code runs rarely, and from a cold cache
+            const int pick = is_v ? i8 * VR / 4 : i8;
+            const int64_t mine_r = pick == 0 ? off[0] : pick == 1 ? off[1] : pick == 2 ? off[2] : off[3];
+#pragma unroll
+          for (int ii = 0; ii < 8; ii++) {
+            const int i = i8 * 8 + ii;
+            const int key = is_v ? i * VR + lane / UR : i * 4 + (lane >> 3), u = is_v ? lane % UR : b * 8 + (lane & 7);
+            const int64_t r = __shfl_sync(0xffffffffu, mine_r, key & 31);
+            const T *src = base + (r < 0 ? 0 : r * rs + u * 8);
+            uint8_t *d = dst + (((u & 7) ^ (key & 7)) << 4) + (is_v ? (key >> 4) * G_::VG + (u >> 3) * 2048 + (key & 15) * 128 : key * 128);
+            if (TREE || a.vec) {
+              cp_async16(smem_u32(d), src, r >= 0);
             } else {
-              c.bad = 1;
-              atomicOr(a.err, OPE_PAGE);
+              T e[8];
+#pragma unroll
+              for (int k = 0; k < 8; k++) e[k] = r >= 0 ? src[k] : from_f<T>(0.f);
+              *(uint4 *)d = *(uint4 *)e;
             }
           }
-          if (g.ts.cut && lt == 0) atomicOr(a.err, OPE_PAGE);
-        } else if (pbegin + sl < pend) {
-          o = (uint32_t)(pbegin + sl);
-        }
-        c.rowoff[tile & 1][lt] = o;
-      }
-      named_bar(4, LD);
-    };
-    auto rows_of = [&](bool is_v, int tile, int hk) {
-#pragma unroll
-      for (int i = 0; i < NR; i++) {
-        const uint32_t o = c.rowoff[tile & 1][r0 + i * RSTEP];
-        const T *p;
-        if constexpr (TREE) p = (const T *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + hk) * HD;
-        else p = (const T *)(is_v ? a.v : a.k) + (int64_t)o * (is_v ? a.vrow : a.krow) + hk * (is_v ? a.vhead : a.khead);
-        row_p[i] = o == NONE ? nullptr : p + u0 * 8;
-      }
-    };
-    // the pieces in the order of their use: K(t0), then K(j), V(j - 1), then V(t1 - 1)
-    Seg g;
-    int si = -1, pj = 0, pb = 0;
-    bool is_v = false, more = false;
-    auto advance = [&]() -> bool {
-      if (more && ++pb == NP) {
-        pb = 0;
-        if (!is_v && pj > g.t0) {
-          is_v = true;
-        } else {
-          is_v = ++pj == g.t1;
-          more = pj <= g.t1;
+          }
+          cp_async_commit();
+          cp_async_wait<0>();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c.full[slot]);
         }
       }
-      if (!more) {
-        if (!next(g)) return false;
-        si++;
-        pj = g.t0;
-        pb = 0;
-        is_v = false;
-        more = true;
-      }
-      if (pb == 0) {
-        if (!is_v) offsets(g, pj);
-        rows_of(is_v, is_v ? pj - 1 : pj, g.hk);
-      }
-      return true;
-    };
-    int slot = 0, par = 1;  // the first pass over the ring waits for nothing
-    auto step = [&]() {
+      if (++turn == LOAD_WARPS) turn = 0;
       if (++slot == NS) {
         slot = 0;
         par ^= 1;
       }
     };
-    if constexpr (F32) {
-      // a thread's four units of a piece are in registers: each is loaded for the next piece as soon as it is
-      // split and stored for this one
+    Seg g;
+    while (next(g)) {
+      if (TREE && g.ts.cut && lane == 0) atomicOr(a.err, OPE_PAGE);
+      // K(t0), then K(j), V(j - 1), then V(t1 - 1)
+      for (int j = g.t0; j <= g.t1; j++) {
+        if (j < g.t1)
+          for (int b = 0; b < NP; b++) put(g, false, j, b);
+        if (j > g.t0)
+          for (int b = 0; b < NP; b++) put(g, true, j - 1, b);
+      }
+    }
+    if (c.abort) {  // copies may still be landing: a millisecond is far beyond any of them
+      const long long t0 = cycles_now();
+      while (cycles_now() - t0 < 2000000ll) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ loads, f32
+    const int lt = tid - 288;
+    // A thread takes 8-dim units of the rows lt/8, lt/8 + 32, ... of a tile: for K piece b the block b of all of
+    // them, for V piece b every block of those in it.
+    constexpr int RSTEP = LD / 8, NR = TC_KEYS / RSTEP, RV = VK / RSTEP;
+    const int r0 = lt >> 3, u0 = lt & 7, swz = (u0 ^ (r0 & 7)) << 4;
+    // unit i (of NR) of a piece: its row and its block, and its place in the piece
+    auto unit_row = [&](bool is_v, int b, int i) { return is_v ? b * RV + i % RV : i; };
+    auto unit_block = [&](bool is_v, int b, int i) { return is_v ? i / RV : b; };
+    auto unit_at = [&](bool is_v, int i) {
+      const int kr = r0 + (is_v ? i % RV : i) * RSTEP;
+      return swz + (is_v ? (kr >> 4) * G_::VG + (i / RV) * 2048 + (kr & 15) * 128 : kr * 128);
+    };
+    constexpr uint32_t NONE = 0xffffffffu;
+    uint32_t(*const rowoff)[TC_KEYS] = c.rowoff;
+    // Rows of a tile's slots.  The table entries of a tile are read two tiles, and its rows are known one tile before
+    // they are used, so that neither load is waited for.
+    int entry = -1, page = -1;
+    auto look = [&](const Seg &g, int tile) {
+      const int sl = tile * TC_KEYS + lt;
+      entry = -1;
+      if constexpr (TREE) {
+        if (tile < g.w1 && lt < TC_KEYS && sl < g.ts.n) {
+          entry = (int)cwp_entry(a.kv.stride, a.kv.page_size, sl);
+          if (entry >= 0) page = a.kv.table[(int64_t)g.s * a.kv.stride + entry];
+        }
+      }
+    };
+    auto note = [&](const Seg &g, int tile) {
+      if (tile >= g.w1 || lt >= TC_KEYS) return;
+      const int sl = tile * TC_KEYS + lt;
+      uint32_t o = NONE;
+      if constexpr (TREE) {
+        if (sl < g.ts.n) {
+          const int64_t x = entry < 0 ? -1 : cwp_row_in(page, entry, a.kv.n_pages, a.kv.page_size, sl);
+          if (x >= 0) {
+            o = (uint32_t)x;
+          } else {
+            c.bad = 1;
+            atomicOr(a.err, OPE_PAGE);
+          }
+        }
+      } else if (pbegin + sl < pend) {
+        o = (uint32_t)(pbegin + sl);
+      }
+      rowoff[tile & 3][lt] = o;
+      if (o != NONE) {  // too few registers to have much in flight: let the L2 fetch it
+        const char *kp, *vp;
+        if constexpr (TREE) {
+          const int64_t at = ((int64_t)o * a.nkv + g.hk) * HD;
+          kp = (const char *)((const T *)a.kv.k + at);
+          vp = (const char *)((const T *)a.kv.v + at);
+        } else {
+          kp = (const char *)((const T *)a.k + (int64_t)o * a.krow + g.hk * a.khead);
+          vp = (const char *)((const T *)a.v + (int64_t)o * a.vrow + g.hk * a.vhead);
+        }
+#pragma unroll
+        for (int d = 0; d < HD * 4; d += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(kp + d));
+#pragma unroll
+        for (int d = 0; d < HD * 4; d += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(vp + d));
+      }
+    };
+    // the row of unit i of a piece, and where the unit is
+    auto row_at = [&](bool is_v, int tile, int b, int i) { return rowoff[tile & 3][r0 + unit_row(is_v, b, i) * RSTEP]; };
+    auto source = [&](const Seg &g, bool is_v, uint32_t o, int b, int i) -> const T * {
+      const int u = unit_block(is_v, b, i) * 64 + u0 * 8;
+      if constexpr (TREE) return (const T *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + g.hk) * HD + u;
+      else return (const T *)(is_v ? a.v : a.k) + (int64_t)o * (is_v ? a.vrow : a.krow) + g.hk * (is_v ? a.vhead : a.khead) + u;
+    };
+    // to be called for the tiles [w0, w1) of a segment in order
+    auto tile_rows = [&](const Seg &g, int tile) {
+      if (tile == g.w0) {
+        named_bar(4, LD);  // the segment before is through with rowoff
+        if (TREE && g.ts.cut && lt == 0) atomicOr(a.err, OPE_PAGE);
+        look(g, tile);
+        note(g, tile);
+        look(g, tile + 1);
+      }
+      note(g, tile + 1);
+      look(g, tile + 2);
+      named_bar(4, LD);
+    };
+    {
+      // the pieces in the order of their use: K(t0), then K(j), V(j - 1), then V(t1 - 1)
+      Seg g;
+      int si = -1, pj = 0, pb = 0;
+      bool is_v = false, more = false;
+      auto advance = [&]() -> bool {
+        if (more && ++pb == NP) {
+          pb = 0;
+          if (!is_v && pj > g.t0) {
+            is_v = true;
+          } else {
+            is_v = ++pj == g.t1;
+            more = pj <= g.t1;
+          }
+        }
+        if (!more) {
+          if (!next(g)) return false;
+          si++;
+          pj = g.t0;
+          pb = 0;
+          is_v = false;
+          more = true;
+        }
+        if (pb == 0 && !is_v) tile_rows(g, pj);
+        return true;
+      };
+      int slot = 0, par = 1;  // the first pass over the ring waits for nothing
+      auto step = [&]() {
+        if (++slot == NS) {
+          slot = 0;
+          par ^= 1;
+        }
+      };
+      // a thread's four units of a piece are in registers; the next piece's are loaded while the MMAs take this one
       float x[4][8];
       const bool vec = TREE || a.vec;
-      // fixed i: the row of a unit depends on the piece only through b, which a switch over few values resolves
       auto load = [&](int i) {
-        const float *src = nullptr;
-        if (!is_v) {
-          src = (const float *)row_p[i];
-        } else {
-#pragma unroll
-          for (int r = 0; r < NR; r++)
-            if (r == unit_row(true, pb, i)) src = (const float *)row_p[r];
-        }
-        if (!src) {
+        const uint32_t o = row_at(is_v, is_v ? pj - 1 : pj, pb, i);
+        const float *src = (const float *)source(g, is_v, o, pb, i);
+        if (o == NONE) {
 #pragma unroll
           for (int k = 0; k < 8; k++) x[i][k] = 0.f;
         } else {
-          src += unit_block(is_v, pb, i) * 64;
           if (vec) {
             *(float4 *)x[i] = *(const float4 *)src;
             *(float4 *)(x[i] + 4) = *(const float4 *)(src + 4);
@@ -904,84 +1077,41 @@ __global__ void __launch_bounds__(Geo<TY, HD>::threads(TMA), 1)
           for (int k = 0; k < 4; k++) split2(x[i][2 * k] * f, x[i][2 * k + 1] * f, hi[k], lo[k]);
           *(uint4 *)(ring + s_hi * PIECE + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4 *)(ring + s_lo * PIECE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          if (have) load(i);
         }
-        fence_proxy_async_smem();
+        fence_proxy_async_smem();  // waits for loads too: before the next ones
         mbar_arrive(&c.full[s_hi]);
         mbar_arrive(&c.full[s_lo]);
-      }
-    } else {
-      constexpr int D = 5;  // pieces in flight per thread
-      static_assert(D < NS, "a piece in flight needs its slot");
-      int done = 0, issued = 0;
-      auto finish = [&]() {  // this thread's part of the oldest piece in flight has landed
-        fence_proxy_async_smem();
-        mbar_arrive(&c.full[done % NS]);
-        done++;
-      };
-      while (advance()) {
-        wait(&c.empty[slot], par);
-        const uint32_t base = smem_u32(ring + slot * PIECE);
-        auto piece = [&](auto v_const, auto b_const) {  // both known: row_p stays in registers
-          constexpr bool V = decltype(v_const)::value;
-          constexpr int B = decltype(b_const)::value;
+        if (have) {
 #pragma unroll
-          for (int i = 0; i < NR; i++) {
-            const T *src = row_p[unit_row(V, B, i)];
-            const bool ok = src != nullptr;
-            src = ok ? src + unit_block(V, B, i) * 64 : (const T *)(TREE ? a.kv.k : a.k);
-            const uint32_t dst = base + unit_at(V, i);
-            if (TREE || a.vec) {
-              cp_async16(dst, src, ok);
-            } else {
-              T e[8];
-#pragma unroll
-              for (int k = 0; k < 8; k++) e[k] = ok ? src[k] : from_f<T>(0.f);
-              const uint4 w = *(uint4 *)e;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                           : "memory");
-            }
-          }
-        };
-        auto of_kind = [&](auto v_const) {
-          if (NP == 1 || pb == 0) piece(v_const, std::integral_constant<int, 0>());
-          else if (NP == 2 || pb == 1) piece(v_const, std::integral_constant<int, NP >= 2 ? 1 : 0>());
-          else if (pb == 2) piece(v_const, std::integral_constant<int, NP >= 4 ? 2 : 0>());
-          else piece(v_const, std::integral_constant<int, NP >= 4 ? 3 : 0>());
-        };
-        if (is_v) of_kind(std::true_type());
-        else of_kind(std::false_type());
-        cp_async_commit();
-        issued++;
-        step();
-        if (issued - done > D) {
-          cp_async_wait<D>();
-          finish();
+          for (int i = 0; i < 4; i++) load(i);
         }
       }
-      cp_async_wait<0>();
-      while (done < issued) finish();
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }
 }
 
-// Joins the parts of a row whose slots were split over CTAs: one warp per row,
-// parts in CTA order.  Grid (sequence, kv head, groups of 8 rows).
+// Joins the parts of the rows whose slots were split over CTAs.  Grid
+// (sequence, kv head, groups of `rows` rows); a CTA takes its rows one after
+// another, its threads as groups of HD/4 that take every NG-th part of the row
+// and four dims each, and adds the groups in order.
 template <int TY, int HD>
-__global__ void __launch_bounds__(256) tc_combine_kernel(const __grid_constant__ AttnOp a) {
+__global__ void __launch_bounds__(256) tc_combine_kernel(const __grid_constant__ AttnOp a, int rows) {
   using T = typename TypeOf<TY>::T;
+  constexpr int TG = HD / 4, NG = 256 / TG;
+  __shared__ float w[TC_CTAS + 8];
+  __shared__ float4 acc_s[256];
+  __shared__ float red_m[8], red_l[8];
   pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, s = blockIdx.x, hk = blockIdx.y, G = a.nh / a.nkv;
-  const int item = blockIdx.z * 8 + (threadIdx.x >> 5);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x, hk = blockIdx.y, G = a.nh / a.nkv;
   const TreeSeq q = tree_seq(a, s);
-  if (item >= q.live * G) return;
+  const int i0 = blockIdx.z * rows, i1 = min(q.live * G, i0 + rows);
+  if (i0 >= i1) return;
   int64_t before = 0, total = 0;
   for (int i = lane; i < a.n_seq; i += 32) {
     const int64_t n = seq_units(a, i);
@@ -994,58 +1124,84 @@ __global__ void __launch_bounds__(256) tc_combine_kernel(const __grid_constant__
     total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   const int C = a.n_cta, nt = tree_tiles(q.n), mts = (q.live * G + TC_ROWS - 1) / TC_ROWS;
-  const int mt = item / TC_ROWS, r = item % TC_ROWS;
-  const int64_t ua = before + (int64_t)(hk * mts + mt) * nt, ub = ua + nt;
-  const int c0 = (int)(((ua + 1) * C - 1) / total), c1 = (int)((ub * C - 1) / total);
-  if (c0 == c1) return;  // written by its CTA
-  // (max, sum) of part c; an empty CTA has none
-  auto part_row = [&](int cc) -> int64_t {
-    const int64_t x0 = total * cc / C, x1 = total * (cc + 1) / C;
-    return x0 == x1 ? -1 : ((int64_t)cc * 2 + (ua >= x0)) * a.part_rows + r;
-  };
-  float m = -INFINITY;
-  for (int cc = c0 + lane; cc <= c1; cc += 32) {
-    const int64_t p = part_row(cc);
-    if (p >= 0) m = fmaxf(m, a.ml[2 * p]);
-  }
-  m = warp_max(m);
-  constexpr int DL = HD / 32;
-  float l = 0.f, acc[DL];
-#pragma unroll
-  for (int i = 0; i < DL; i++) acc[i] = 0.f;
-  for (int cb = c0; cb <= c1; cb += 32) {
-    const int64_t p = cb + lane <= c1 ? part_row(cb + lane) : -1;
-    float w = 0.f, lp = 0.f;
-    if (p >= 0) {
-      const float mp = a.ml[2 * p];
+  // first unit of CTA c: floor(total c / C)
+  const int64_t tq = total / C;
+  const int tr = (int)(total - tq * C);
+  auto first_unit = [&](int cc) { return tq * cc + (tr * cc) / C; };
+  pdl_wait();  // the lengths are older than the kernel before, which ends its own wait before this one starts
+  int mt = -1, c0 = 0, c1 = 0;
+  int64_t ua = 0;
+  for (int item = i0; item < i1; item++) {
+    if (item / TC_ROWS != mt) {
+      mt = item / TC_ROWS;
+      ua = before + (int64_t)(hk * mts + mt) * (nt + SEG_COST) + SEG_COST;  // the segment's first tile
+      c0 = (int)(((ua + 1) * C - 1) / total);
+      c1 = (int)(((ua + nt) * C - 1) / total);
+    }
+    if (c0 == c1) continue;  // written by its CTA
+    const int r = item - mt * TC_ROWS, np = c1 - c0 + 1;
+    // weight of part c0 + tid (an empty CTA has none; np <= TC_CTAS < 256)
+    auto part_row = [&](int i) -> int64_t { return ((int64_t)(c0 + i) * 2 + (ua >= first_unit(c0 + i))) * a.part_rows + r; };
+    float mp = -INFINITY, lp = 0.f;
+    if (tid < np && first_unit(c0 + tid) != first_unit(c0 + tid + 1)) {
+      const int64_t p = part_row(tid);
+      mp = a.ml[2 * p];
       lp = a.ml[2 * p + 1];
-      w = mp == -INFINITY ? 0.f : ex2(mp - m);
-      if (lp != lp) w = 1.f;
     }
-    l += warp_sum(w * lp);
-    const int n = min(32, c1 - cb + 1);
+    const float mw = warp_max(mp);
+    if (lane == 0) red_m[warp] = mw;
+    __syncthreads();
+    float m = red_m[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) m = fmaxf(m, red_m[i]);
+    float wt = mp == -INFINITY ? 0.f : ex2(mp - m);
+    if (lp != lp) wt = 1.f;
+    if (tid < np) w[tid] = wt;
+    const float lw = warp_sum(wt * lp);
+    if (lane == 0) red_l[warp] = lw;
+    __syncthreads();
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) l += red_l[i];
+    const int g = tid / TG, d = (tid % TG) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = 0; i < n; i++) {
-      const int64_t pi = __shfl_sync(0xffffffffu, p, i);
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      if (pi < 0 || wi == 0.f) continue;
-      const float *x = a.part + pi * HD + lane * DL;
-#pragma unroll
-      for (int d = 0; d < DL; d++) acc[d] = fmaf(wi, x[d], acc[d]);
+    for (int i = g; i < np; i += NG) {
+      const float wi = w[i];
+      if (wi != 0.f) {  // a part of no weight may never have been written
+        const float4 x = *(const float4 *)(a.part + part_row(i) * HD + d);
+        acc.x = fmaf(wi, x.x, acc.x);
+        acc.y = fmaf(wi, x.y, acc.y);
+        acc.z = fmaf(wi, x.z, acc.z);
+        acc.w = fmaf(wi, x.w, acc.w);
+      }
     }
-  }
-  const int t = item / G, h = hk * G + item - t * G;
-  const int64_t row = (int64_t)s * a.T + t;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  bool bad = !(l < INFINITY);
-  T *o = (T *)a.o + row * a.orow + h * a.ohead + lane * DL;
+    acc_s[tid] = acc;
+    __syncthreads();
+    const int t = item / G, h = hk * G + item - t * G;
+    const int64_t row = (int64_t)s * a.T + t;
+    bool bad = false;
+    if (tid < TG) {
 #pragma unroll
-  for (int d = 0; d < DL; d++) {
-    const float x = l == 0.f ? 0.f : acc[d] * inv;
-    bad |= !(fabsf(x) < INFINITY);
-    o[d] = from_f<T>(x);
+      for (int i = 1; i < NG; i++) {
+        const float4 x = acc_s[tid + i * TG];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      bad = !(l < INFINITY);
+      T *o = (T *)a.o + row * a.orow + h * a.ohead + d;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        bad |= !(fabsf(f[i]) < INFINITY);
+        o[i] = from_f<T>(l == 0.f ? 0.f : f[i]);
+      }
+    }
+    if (__syncthreads_or(bad) && warp == 0) exact_row<T, HD, true>(a, s, t, 0, (int)row, h);
   }
-  if (__any_sync(0xffffffffu, bad)) exact_row<T, HD, true>(a, s, t, 0, (int)row, h);
 }
 
 // ------------------------------------------------------------------ host
@@ -1070,45 +1226,50 @@ bool make_map(CUtensorMap *m, bool bf16, const void *p, int64_t row, int64_t hea
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int TY, int HD, bool TREE, bool TMA>
-cudaError_t configure_one() {
-  return cudaFuncSetAttribute(attn_tc_kernel<TY, HD, TREE, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Geo<TY, HD>::SMEM);
-}
 template <int TY, int HD>
 cudaError_t configure_hd() {
-  if constexpr (TY != TY_F32) CW_TRY((configure_one<TY, HD, false, true>()));
-  CW_TRY((configure_one<TY, HD, false, false>()));
-  CW_TRY((configure_one<TY, HD, true, false>()));
+  CW_TRY(cudaFuncSetAttribute(attn_tc_kernel<TY, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<TY, HD>::SMEM));
+  CW_TRY(cudaFuncSetAttribute(attn_tc_kernel<TY, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<TY, HD>::SMEM));
   return carveout_max(tc_combine_kernel<TY, HD>);
+}
+
+// Tensor maps of K and V; false where their rows cannot be addressed so.
+template <int TY, int HD>
+bool make_maps(CUtensorMap &mk, CUtensorMap &mv, const void *k, int64_t krow, int64_t khead, const void *v, int64_t vrow,
+               int64_t vhead, int nkv, int n_rows, int kbox) {
+  memset(&mk, 0, sizeof mk);
+  memset(&mv, 0, sizeof mv);
+  return TY != TY_F32 && kbox >= 16 && make_map(&mk, TY == TY_BF16, k, krow, khead, HD, nkv, n_rows, kbox, 1) &&
+         make_map(&mv, TY == TY_BF16, v, vrow, vhead, HD, nkv, n_rows, 16, HD / 64);
 }
 
 template <int TY, int HD>
 cudaError_t prompt_hd(AttnOp a, cudaStream_t st) {
   CUtensorMap mk, mv;
+  using G = Geo<TY, HD>;
   const int64_t tiles = (int64_t)a.n_rows / TC_ROWS + a.n_seq;
   if (tiles * a.nh > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  const dim3 grid((unsigned)(tiles * a.nh));
-  using G = Geo<TY, HD>;
-  if constexpr (TY != TY_F32) {
-    if (make_map(&mk, TY == TY_BF16, a.k, a.krow, a.khead, HD, a.nkv, a.n_rows, TC_KEYS, 1) &&
-        make_map(&mv, TY == TY_BF16, a.v, a.vrow, a.vhead, HD, a.nkv, a.n_rows, G::VK, G::CB))
-      return launch_pdl(attn_tc_kernel<TY, HD, false, true>, grid, G::threads(true), G::SMEM, st, a, mk, mv);
-  }
-  memset(&mk, 0, sizeof mk);
-  memset(&mv, 0, sizeof mv);
   const int al = TY == TY_F32 ? 4 : 8;
   a.vec = ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.krow | a.khead | a.vrow | a.vhead) % al == 0;
-  return launch_pdl(attn_tc_kernel<TY, HD, false, false>, grid, G::threads(false), G::SMEM, st, a, mk, mv);
+  const int kbox = make_maps<TY, HD>(mk, mv, a.k, a.krow, a.khead, a.v, a.vrow, a.vhead, a.nkv, a.n_rows, TC_KEYS) ? TC_KEYS : 0;
+  return launch_pdl(attn_tc_kernel<TY, HD, false>, dim3((unsigned)(tiles * a.nh)), G::THREADS, G::SMEM, st, a, mk, mv, kbox);
 }
 
 template <int TY, int HD>
 cudaError_t tree_hd(const AttnOp &a, cudaStream_t st) {
-  static const CUtensorMap none = {};
+  CUtensorMap mk, mv;
   using G = Geo<TY, HD>;
-  CW_TRY(launch_pdl(attn_tc_kernel<TY, HD, true, false>, dim3(a.n_cta), G::threads(false), G::SMEM, st, a, none, none));
+  int kbox = a.kv.page_size & -a.kv.page_size;
+  kbox = kbox > TC_KEYS ? TC_KEYS : kbox;
+  const int64_t row = (int64_t)a.nkv * HD;
+  if (!make_maps<TY, HD>(mk, mv, a.kv.k, row, HD, a.kv.v, row, HD, a.nkv, a.kv.n_pages * a.kv.page_size, kbox)) kbox = 0;
+  CW_TRY(launch_pdl(attn_tc_kernel<TY, HD, true>, dim3(a.n_cta), G::THREADS, G::SMEM, st, a, mk, mv, kbox));
   if (tree_tiles(a.max_len) == 1) return cudaSuccess;  // no segment can be split
-  return launch_pdl(tc_combine_kernel<TY, HD>, dim3(a.n_seq, a.nkv, (a.T * (a.nh / a.nkv) + 7) / 8), 256, 0, st, a);
+  // rows one after another in a CTA once there is more than a wave of them
+  const int per = a.T * (a.nh / a.nkv);
+  const int64_t want = ((int64_t)a.n_seq * a.nkv * per + 8 * a.n_cta - 1) / (8 * a.n_cta);
+  const int rows = (int)(want < 1 ? 1 : want > per ? per : want);
+  return launch_pdl(tc_combine_kernel<TY, HD>, dim3(a.n_seq, a.nkv, (per + rows - 1) / rows), 256, 0, st, a, rows);
 }
 
 template <int TY>

@@ -13,16 +13,23 @@
 #define CWP_FN static inline
 #endif
 
+// Place in a sequence's table row of the page that holds `slot`, or -1.
+CWP_FN int64_t cwp_entry(int table_stride, int page_size, int64_t slot) {
+  if (slot < 0 || slot >= (int64_t)table_stride * page_size) return -1;
+  // in range, slot / page_size < table_stride: 32-bit arithmetic where it can be
+  return slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
+}
+// Pool row of `slot` whose table entry (at cwp_entry) is `page`, or -1 when that is no page of the pool.
+CWP_FN int64_t cwp_row_in(int page, int64_t entry, int n_pages, int page_size, int64_t slot) {
+  if (page < 0 || page >= n_pages) return -1;
+  return (int64_t)page * page_size + (slot - entry * page_size);
+}
 // Pool row (page * page_size + slot in the page) of a sequence's `slot`, or
 // -1 when the slot lies outside the table row or its page id outside
 // [0, n_pages).  64 bits: a pool may hold more than 2^31 rows' elements.
 CWP_FN int64_t cwp_row(const int *table_row, int table_stride, int n_pages, int page_size, int64_t slot) {
-  if (slot < 0 || slot >= (int64_t)table_stride * page_size) return -1;
-  // in range, slot / page_size < table_stride: 32-bit arithmetic where it can be
-  const int64_t p = slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)page_size) : slot / page_size;
-  const int page = table_row[p];
-  if (page < 0 || page >= n_pages) return -1;
-  return (int64_t)page * page_size + (slot - p * page_size);
+  const int64_t e = cwp_entry(table_stride, page_size, slot);
+  return e < 0 ? -1 : cwp_row_in(table_row[e], e, n_pages, page_size, slot);
 }
 
 // Slot of the i-th set bit (from the lowest) of a 64-bit keep mask; -1 past the last.

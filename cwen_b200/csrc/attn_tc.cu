@@ -454,47 +454,69 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
       };
       const bool first = g.t0 == g.w0, last = g.t1 == g.w1;  // window of the segment
       if (first) {
-      for (int i = tid; i < 128 * CB * 8; i += 256) {
-        const int rr = i / (CB * 8), u = i % (CB * 8);
-        int64_t row;
-        int h, t;
-        const bool have = place(rr, row, h, t);
-        uint8_t *dst = qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4);
-        const T *src = (const T *)a.q + (have ? row * a.qrow + h * a.qhead + u * 8 : 0);
         if constexpr (F32) {
-          float x[8];
-          if (qvec && have) {
-            *(float4 *)x = *(const float4 *)src;
-            *(float4 *)(x + 4) = *(const float4 *)(src + 4);
-          } else {
+          constexpr int UB = CB < 4 ? CB : 4;  // units on their way at once
+#pragma unroll 1
+          for (int i0 = tid; i0 < 128 * CB * 8; i0 += 256 * UB) {
+            float x[UB][8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = have ? src[k] : 0.f;
+            for (int j = 0; j < UB; j++) {
+              const int i = i0 + 256 * j, rr = i / (CB * 8), u = i % (CB * 8);
+              int64_t row;
+              int h, t;
+              const bool have = place(rr, row, h, t);
+              const float *src = (const float *)a.q + (have ? row * a.qrow + h * a.qhead + u * 8 : 0);
+#pragma unroll
+              for (int k = 0; k < 8; k++) x[j][k] = 0.f;
+              if (have && qvec) {
+                *(float4 *)x[j] = *(const float4 *)src;
+                *(float4 *)(x[j] + 4) = *(const float4 *)(src + 4);
+              } else if (have) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[j][k] = src[k];
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < UB; j++) {
+              const int i = i0 + 256 * j, rr = i / (CB * 8), u = i % (CB * 8);
+              uint8_t *dst = qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4);
+              float mx = 0.f;
+#pragma unroll
+              for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[j][k]));
+#pragma unroll
+              for (int k = 1; k < CB * 8; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+              const int e = scale_exp(mx);
+              const float f = a.scale < 0.f ? -exp2_int(e) : exp2_int(e);
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int k = 0; k < 4; k++) split2(x[j][2 * k] * f, x[j][2 * k + 1] * f, hi[k], lo[k]);
+              *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *(uint4 *)(dst + G_::Q_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              if (u == 0) c.qe[rr] = e;
+            }
           }
-          float mx = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
-#pragma unroll
-          for (int k = 1; k < CB * 8; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-          const int e = scale_exp(mx);
-          const float f = a.scale < 0.f ? -exp2_int(e) : exp2_int(e);
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) split2(x[2 * k] * f, x[2 * k + 1] * f, hi[k], lo[k]);
-          *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *(uint4 *)(dst + G_::Q_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          if (u == 0) c.qe[rr] = e;
-        } else if (qvec) {
-          cp_async16(smem_u32(dst), src, have);
         } else {
-          T e[8];
+#pragma unroll 4
+          for (int i = tid; i < 128 * CB * 8; i += 256) {
+            const int rr = i / (CB * 8), u = i % (CB * 8);
+            int64_t row;
+            int h, t;
+            const bool have = place(rr, row, h, t);
+            uint8_t *dst = qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4);
+            const T *src = (const T *)a.q + (have ? row * a.qrow + h * a.qhead + u * 8 : 0);
+            if (qvec) {
+              cp_async16(smem_u32(dst), src, have);
+            } else {
+              T e[8];
 #pragma unroll
-          for (int k = 0; k < 8; k++) {
-            const float x = have ? to_f<T>(src[k]) : 0.f;
-            e[k] = from_f<T>(a.scale < 0.f ? -x : x);  // exact: |scale| is used below
+              for (int k = 0; k < 8; k++) {
+                const float x = have ? to_f<T>(src[k]) : 0.f;
+                e[k] = from_f<T>(a.scale < 0.f ? -x : x);  // exact: |scale| is used below
+              }
+              *(uint4 *)dst = *(uint4 *)e;
+            }
           }
-          *(uint4 *)dst = *(uint4 *)e;
         }
-      }
       }
       int64_t row;
       int h, t;
@@ -947,21 +969,6 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
         o = (uint32_t)(pbegin + sl);
       }
       rowoff[tile & 3][lt] = o;
-      if (o != NONE) {  // too few registers to have much in flight: let the L2 fetch it
-        const char *kp, *vp;
-        if constexpr (TREE) {
-          const int64_t at = ((int64_t)o * a.nkv + g.hk) * HD;
-          kp = (const char *)((const T *)a.kv.k + at);
-          vp = (const char *)((const T *)a.kv.v + at);
-        } else {
-          kp = (const char *)((const T *)a.k + (int64_t)o * a.krow + g.hk * a.khead);
-          vp = (const char *)((const T *)a.v + (int64_t)o * a.vrow + g.hk * a.vhead);
-        }
-#pragma unroll
-        for (int d = 0; d < HD * 4; d += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(kp + d));
-#pragma unroll
-        for (int d = 0; d < HD * 4; d += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(vp + d));
-      }
     };
     // the row of unit i of a piece, and where the unit is
     auto row_at = [&](bool is_v, int tile, int b, int i) { return rowoff[tile & 3][r0 + unit_row(is_v, b, i) * RSTEP]; };

@@ -31,16 +31,3 @@ CWP_FN int64_t cwp_row(const int *table_row, int table_stride, int n_pages, int 
   const int64_t e = cwp_entry(table_stride, page_size, slot);
   return e < 0 ? -1 : cwp_row_in(table_row[e], e, n_pages, page_size, slot);
 }
-
-// Slot of the i-th set bit (from the lowest) of a 64-bit keep mask; -1 past the last.
-CWP_FN int cwp_nth_bit(uint64_t m, int i) {
-  for (; m; m &= m - 1)
-    if (i-- == 0) {
-#ifdef __CUDA_ARCH__
-      return __ffsll((long long)m) - 1;
-#else
-      return __builtin_ctzll(m);
-#endif
-    }
-  return -1;
-}

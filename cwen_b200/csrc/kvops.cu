@@ -8,6 +8,13 @@
 // the rotation are fp32.
 // append: the same rotation on K rows on their way into the pages, V beside it.
 // compact: the rows of an accepted path move down to consecutive slots.
+//
+// All three are bound by HBM (short calls by their launch).  Measured on B200:
+// rope of 16384 rows of 32 x 128 bf16 50 us (5.4 TB/s); append of 32768 rows of
+// 4 x 256, f32 into bf16, 91 us (4.4 TB/s: the look-ups of place and angle come
+// before a CTA's first store); compaction of 64 sequences in 16 bf16 layers 39 us
+// (5.7 TB/s).  Many small CTAs with one unit per thread in flight beat fewer with
+// four (110-130 us for the append).
 #include <math.h>
 #include <string.h>
 
@@ -170,6 +177,7 @@ __global__ void __launch_bounds__(RT) rows_kernel(const __grid_constant__ RowsAr
 // from slot len + u to len + i <= len + u, so in path order no source lies
 // behind a destination: a thread that owns one 16-byte column of the rows
 // makes its moves in order, loads of a group before its stores.
+// Sixteen moves in flight: 36 us where eight took 54 (64 sequences, 16 layers).
 constexpr int CT = 128, CG = 16;  // threads of a CTA; moves of a group
 __global__ void __launch_bounds__(CT) compact_kernel(uint4 *k, uint4 *v, int n_layer, int64_t layer_cols, int cols,
                                                      const int *table, int stride, int n_pages, int page_size,

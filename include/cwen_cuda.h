@@ -227,7 +227,10 @@ int cwen_cuda_accept_logits(const float *dlogits, int n, int ldl, int B, const i
  *    engine's stream; the legacy default stream is cudaStreamLegacy); calls
  *    do not synchronize or allocate and can be captured into graphs;
  *  - types are CWEN_T_F32, CWEN_T_F16, CWEN_T_BF16; softmax statistics and sums
- *    are fp32, each result is rounded once;
+ *    are fp32, each result is rounded once (attention weights of 16-bit types are
+ *    rounded to the type for the product with V; f32 products keep 22 bits of
+ *    each factor, and of V 2^-33 of the largest value among the 1024 slots that
+ *    are taken together);
  *  - device arrays (lengths, slots, page ids) cannot be checked on the host:
  *    what is out of range is never dereferenced, its rows or slots are left
  *    out, and cwen_cuda_attn_status reports it.

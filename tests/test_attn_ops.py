@@ -404,6 +404,23 @@ def test_prompt_maximum_jumps(cw, t, hd):
     check_prompt(o[0], t, [n], 1, 1, q[0], k[0], v[0], 0.25)
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("first,rest", [(0.0, 1e-4), (1.0, 1e6), (1e6, 1.0), (1e-20, 1e-20), (1e15, 1e15)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_prompt_f32_magnitudes(cw, hd, first, rest, what):
+    """The f32 parts are scaled by what a window's first slots hold: zeros there, values that grow or shrink by a
+    million behind them, tiny and huge ones.  K's stay within scores of a few units by q."""
+    g, n = gen(15), 300
+    q, k, v, o = (rows_of(g, n, 1, hd, F32) for _ in range(4))
+    x = k if what == "k" else v
+    x[0][:128] *= first
+    x[0][128:] *= rest
+    if what == "k":
+        q[0].mul_(1.0 / max(first, rest))
+    run_prompt(cw, F32, [n], 1, 1, hd, None, q, k, v, o)
+    check_prompt(o[0], F32, [n], 1, 1, q[0], k[0], v[0], hd ** -0.5)
+
+
 def test_prompt_malformed_offsets_stay_in_bounds(cw):
     """cu that decreases, is negative or passes n_rows is cut to the rows there are: finite neighbours stay right."""
     g, nh, nkv, hd, n = gen(3), 2, 1, 64, 100

@@ -335,6 +335,10 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
     c.bad = 0;
   }
   if (tid < 4) c.badrows[tid] = 0;
+  if (!F32 && kbox && tid == 9 * 32) {
+    tma_prefetch_map(&mk);
+    tma_prefetch_map(&mv);
+  }
   pdl_wait();
   pdl_trigger();  // after the wait: the joining kernel may read the lengths before its own wait
   if (warp == 0) {  // this CTA's work

@@ -78,6 +78,10 @@ CW_DEV void tma_4d(void *dst, const void *map, int x, int y, int z, int w, uint6
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+// Have a tensor map (a kernel parameter) at hand before its first copy.
+CW_DEV void tma_prefetch_map(const void *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // 16-byte asynchronous copy by this thread, or 16 zero bytes when !valid.
 CW_DEV void cp_async16(uint32_t dst, const void *src, bool valid) {
   const int n = valid ? 16 : 0;

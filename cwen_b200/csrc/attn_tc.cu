@@ -70,15 +70,14 @@ struct Geo {
   static constexpr int NS = F32 ? (HD == 256 ? 5 : HD == 128 ? 9 : 11) : (HD == 256 ? 9 : HD == 128 ? 11 : 12);
   static constexpr int SMEM = Q_BYTES * (F32 ? 2 : 1) + NS * PIECE + 1024;
   static constexpr int LOADERS = F32 ? 256 : 32 * LOAD_WARPS, THREADS = 288 + LOADERS;
+  // Tree: what a segment's start and end cost, in tiles.  31 ragged sequences of 8 kv heads of 128, to 12000 slots: 295 us
+  // with 4, 272 with 6, 256 with 8 and 257 with 12; 4 heads of 256 207, 202, 201, 207; f32 (8 sequences) 197, 209, 209, 229.
+  static constexpr int SEG_COST = F32 ? 4 : HD == 256 ? 6 : 8;
   static constexpr int VG = CB * 2048;       // 16 slots of a V piece: [block][16 slots][128 B]
 };
 // f32: tiles of a window.  Error against 64 bits of a 4100-token prompt and a 12000-token one: 3.1e-6 and 2.3e-6 with 4,
 // 3.7e-6 with 8 (prompt), 4.9e-6 and 5.1e-6 with 16, 6.0e-6 and 1.3e-5 unbroken; a window's end costs about 20000 clocks.
 constexpr int WIN = 8;
-// Tree: what a segment's start and end cost, in tiles.  31 ragged sequences of 8 kv heads: the CTA with six short
-// segments ended at 450k clocks beside 280k of one with two, 395k beside 327k with this.
-constexpr int SEG_COST = 4;
-
 struct Ctl {
   uint64_t full[12], empty[12], s_full[2], p_ready[2], pv_done, q_full, o_free, o_done, drained, tail[LOAD_WARPS];
   int64_t u0, u1;
@@ -106,12 +105,12 @@ struct Seg {
 };
 
 CW_HOST_DEV int tree_tiles(int n) { return (n + TC_KEYS - 1) / TC_KEYS; }
-// Units of a segment: first SEG_COST that stand for its fixed cost, then its tiles.
-CW_HOST_DEV int seg_units(int n) { return tree_tiles(n) + SEG_COST; }
+// Units of a segment: first seg_cost that stand for its fixed cost, then its tiles.
+CW_DEV int seg_units(const AttnOp &a, int n) { return tree_tiles(n) + a.seg_cost; }
 CW_DEV int64_t seq_units(const AttnOp &a, int s) {
   const TreeSeq q = tree_seq(a, s);
   const int G = a.nh / a.nkv;
-  return q.live ? (int64_t)a.nkv * ((q.live * G + TC_ROWS - 1) / TC_ROWS) * seg_units(q.n) : 0;
+  return q.live ? (int64_t)a.nkv * ((q.live * G + TC_ROWS - 1) / TC_ROWS) * seg_units(a, q.n) : 0;
 }
 CW_DEV int64_t warp_scan(int64_t v) {  // inclusive
   const int lane = threadIdx.x & 31;
@@ -148,12 +147,12 @@ struct TreeWalk {
     g.s = s;
     g.hk = hk;
     g.mt = mt;
-    const int end = (int)min((int64_t)seg_units(g.ts.n), t0 + left);  // units [t0, end) of the segment
-    g.t0 = max(t0 - SEG_COST, 0);
-    g.t1 = max(end - SEG_COST, 0);
+    const int end = (int)min((int64_t)seg_units(a, g.ts.n), t0 + left);  // units [t0, end) of the segment
+    g.t0 = max(t0 - a.seg_cost, 0);
+    g.t1 = max(end - a.seg_cost, 0);
     left -= end - t0;
     t0 = 0;
-    if (end == seg_units(g.ts.n) && ++mt * TC_ROWS >= g.ts.live * G) {
+    if (end == seg_units(a, g.ts.n) && ++mt * TC_ROWS >= g.ts.live * G) {
       mt = 0;
       if (++hk == a.nkv) {
         hk = 0;
@@ -385,7 +384,7 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
           if constexpr (TREE) {
             const TreeSeq q = tree_seq(a, i);
             const int64_t rem = u0 - at;
-            const int nt = seg_units(q.n), mts = (q.live * G + TC_ROWS - 1) / TC_ROWS;
+            const int nt = seg_units(a, q.n), mts = (q.live * G + TC_ROWS - 1) / TC_ROWS;
             const int64_t x = rem <= 0x7fffffff ? (uint32_t)rem / (uint32_t)nt : rem / nt;
             c.t00 = (int)(rem - x * nt);
             c.mt0 = (int)x % mts;  // x < n_kv mts
@@ -1163,7 +1162,7 @@ __global__ void __launch_bounds__(256) tc_combine_kernel(const __grid_constant__
   for (int item = i0; item < i1; item++) {
     if (item / TC_ROWS != mt) {
       mt = item / TC_ROWS;
-      ua = before + (int64_t)(hk * mts + mt) * (nt + SEG_COST) + SEG_COST;  // the segment's first tile
+      ua = before + (int64_t)(hk * mts + mt) * (nt + a.seg_cost) + a.seg_cost;  // the segment's first tile
       c0 = (int)(((ua + 1) * C - 1) / total);
       c1 = (int)(((ua + nt) * C - 1) / total);
     }
@@ -1285,9 +1284,10 @@ cudaError_t prompt_hd(AttnOp a, cudaStream_t st) {
 }
 
 template <int TY, int HD>
-cudaError_t tree_hd(const AttnOp &a, cudaStream_t st) {
+cudaError_t tree_hd(AttnOp a, cudaStream_t st) {
   CUtensorMap mk, mv;
   using G = Geo<TY, HD>;
+  a.seg_cost = G::SEG_COST;
   int kbox = a.kv.page_size & -a.kv.page_size;
   kbox = kbox > TC_KEYS ? TC_KEYS : kbox;
   const int64_t row = (int64_t)a.nkv * HD;

@@ -20,7 +20,7 @@ struct AttnOp {
   float scale;
   int vec;                    // prompt: k and v rows are 16-byte aligned
   float *part, *ml;           // tree: partial outputs and their (max, sum)
-  int part_rows, n_cta;
+  int part_rows, n_cta, seg_cost;
   int *err;
 };
 

@@ -671,9 +671,8 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
           }
         }
       }
-      // Q is read no more (f32: it is, by the next window)
-      uint8_t *stage = qs + warp * 2048;
-      if constexpr (F32) stage = c.stage[warp];
+      // Q is read no more, but by another window of the segment
+      uint8_t *const stage = qs + warp * 2048;
       if (warp_live) {
 #pragma unroll 1
         for (int k = 0; k < HD / 64; k++) {
@@ -685,20 +684,24 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
           if constexpr (F32) {
             float *dst = part ? part + col : (float *)o;
             const bool v4 = part || ovec;
+            auto emit = [&](auto units, uint8_t *st) {
+              constexpr int U = decltype(units)::value;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t old[8];
-              float f[8];
-              if (!first) fetch_rows<2>(stage, old, dst + i, have, v4);
+              for (int i = 0; i < 32; i += 4 * U) {
+                uint32_t old[4 * U];
+                float f[4 * U];
+                if (!first) fetch_rows<U>(st, old, dst + i, have, v4);
 #pragma unroll
-              for (int d = 0; d < 8; d++) {
-                f[d] = __uint_as_float(x[i + d]) * f_new;
-                if (!first) f[d] = fmaf(__uint_as_float(old[d]), f_old, f[d]);
-                f[d] = l == 0.f ? 0.f : f[d] * inv;
-                bad |= !(fabsf(f[d]) < INFINITY);
+                for (int d = 0; d < 4 * U; d++) {
+                  f[d] = __uint_as_float(x[i + d]) * f_new;
+                  if (!first) f[d] = fmaf(__uint_as_float(old[d]), f_old, f[d]);
+                  f[d] = l == 0.f ? 0.f : f[d] * inv;
+                  bad |= !(fabsf(f[d]) < INFINITY);
+                }
+                flush_rows<U>(st, (const uint32_t *)f, dst + i, have, v4);
               }
-              flush_rows<2>(stage, (const uint32_t *)f, dst + i, have, v4);
-            }
+            };
+            emit(std::integral_constant<int, 2>(), c.stage[warp]);
           } else {
             float f[32];
 #pragma unroll
@@ -1043,34 +1046,49 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
       };
       // a thread's four units of a piece are in registers; the next piece's are loaded while the MMAs take this one
       float x[4][8];
-      const bool vec = TREE || a.vec;
-      auto load = [&](int i) {
-        const uint32_t o = row_at(is_v, is_v ? pj - 1 : pj, pb, i);
-        const float *src = (const float *)source(g, is_v, o, pb, i);
-        if (o == NONE) {
+      unsigned gone = 0;  // units whose slot is not there: read from a row that is, made zero below
+      auto load = [&]() {
+        const int tile = is_v ? pj - 1 : pj;
+        const float *src[4];
+        gone = 0;
 #pragma unroll
-          for (int k = 0; k < 8; k++) x[i][k] = 0.f;
-        } else {
-          if (vec) {
-            *(float4 *)x[i] = *(const float4 *)src;
-            *(float4 *)(x[i] + 4) = *(const float4 *)(src + 4);
-          } else {
+        for (int i = 0; i < 4; i++) {
+          const uint32_t o = row_at(is_v, tile, pb, i);
+          if (o == NONE) gone |= 1u << i;
+          src[i] = (const float *)source(g, is_v, o == NONE ? (TREE ? 0 : pbegin) : o, pb, i);
+        }
+        if (a.vec == 2) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[i][k] = src[k];
+          for (int i = 0; i < 4; i++) ld_global_f8(src[i], x[i]);
+        } else if (a.vec) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            *(float4 *)x[i] = *(const float4 *)src[i];
+            *(float4 *)(x[i] + 4) = *(const float4 *)(src[i] + 4);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[i][k] = src[i][k];
         }
       };
       float fk = 1.f, fv = 1.f;
       bool have = advance();
-      if (have) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) load(i);
-      }
+      if (have) load();
       while (have) {
         const bool v = is_v, first = (v ? pj - 1 : pj) == g.t0 && pb == 0;
         const int wi = si & 7;
         have = advance();
         int e = 0;
+        if (gone) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if ((gone >> i) & 1) {
+#pragma unroll
+              for (int k = 0; k < 8; k++) x[i][k] = 0.f;
+            }
+        }
         if (first) {
           float mx = 0.f;
 #pragma unroll
@@ -1106,10 +1124,7 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
         fence_proxy_async_smem();  // waits for loads too: before the next ones
         mbar_arrive(&c.full[s_hi]);
         mbar_arrive(&c.full[s_lo]);
-        if (have) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) load(i);
-        }
+        if (have) load();
       }
     }
   }
@@ -1279,6 +1294,7 @@ cudaError_t prompt_hd(AttnOp a, cudaStream_t st) {
   if (tiles * a.nh > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const int al = TY == TY_F32 ? 4 : 8;
   a.vec = ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.krow | a.khead | a.vrow | a.vhead) % al == 0;
+  if (a.vec && ((uintptr_t)a.k | (uintptr_t)a.v) % 32 == 0 && (a.krow | a.khead | a.vrow | a.vhead) % 8 == 0) a.vec = 2;
   const int kbox = make_maps<TY, HD>(mk, mv, a.k, a.krow, a.khead, a.v, a.vrow, a.vhead, a.nkv, a.n_rows, TC_KEYS) ? TC_KEYS : 0;
   return launch_pdl(attn_tc_kernel<TY, HD, false>, dim3((unsigned)(tiles * a.nh)), G::THREADS, G::SMEM, st, a, mk, mv, kbox);
 }
@@ -1288,6 +1304,7 @@ cudaError_t tree_hd(AttnOp a, cudaStream_t st) {
   CUtensorMap mk, mv;
   using G = Geo<TY, HD>;
   a.seg_cost = G::SEG_COST;
+  a.vec = ((uintptr_t)a.kv.k | (uintptr_t)a.kv.v) % 32 == 0 ? 2 : 1;
   int kbox = a.kv.page_size & -a.kv.page_size;
   kbox = kbox > TC_KEYS ? TC_KEYS : kbox;
   const int64_t row = (int64_t)a.nkv * HD;

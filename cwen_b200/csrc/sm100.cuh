@@ -78,6 +78,13 @@ CW_DEV void tma_4d(void *dst, const void *map, int x, int y, int z, int w, uint6
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+// 32 bytes of global memory at once (32-byte aligned).
+CW_DEV void ld_global_f8(const float *p, float (&x)[8]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "l"(p)
+               : "memory");
+}
 // Have a tensor map (a kernel parameter) at hand before its first copy.
 CW_DEV void tma_prefetch_map(const void *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");

@@ -37,7 +37,7 @@
 // ms, 1.0 PFLOP/s of causal work, bound by the 128 KB of K and V that every SM
 // draws from the L2 per tile; one token over 32767 bf16 slots 44 us (a bare load
 // of its bytes 33 us); 9 f32 nodes over 32495 slots 120 us and f32 prompts of 4100
-// tokens 1.18 ms, both bound by the loaders' split into parts.
+// tokens 0.95 ms, both bound by the loaders' split into parts.
 #include <cuda.h>
 #include <string.h>
 
@@ -70,9 +70,10 @@ struct Geo {
   static constexpr int NS = F32 ? (HD == 256 ? 5 : HD == 128 ? 9 : 11) : (HD == 256 ? 9 : HD == 128 ? 11 : 12);
   static constexpr int SMEM = Q_BYTES * (F32 ? 2 : 1) + NS * PIECE + 1024;
   static constexpr int LOADERS = F32 ? 256 : 32 * LOAD_WARPS, THREADS = 288 + LOADERS;
-  // Tree: what a segment's start and end cost, in tiles.  31 ragged sequences of 8 kv heads of 128, to 12000 slots: 295 us
-  // with 4, 272 with 6, 256 with 8 and 257 with 12; 4 heads of 256 207, 202, 201, 207; f32 (8 sequences) 197, 209, 209, 229.
-  static constexpr int SEG_COST = F32 ? 4 : HD == 256 ? 6 : 8;
+  // Tree: what a segment's start and end cost, in tiles.  31 ragged sequences of 8 kv heads of 128, to 12000 slots, a call
+  // by itself: 295 us with 4, 272 with 6, 256 with 8 and 257 with 12 (one after another 270 with each); 4 heads of 256
+  // one after another 214 with 4, 218 with 6; f32 (8 sequences) 197, 209, 209, 229 with 4, 6, 8, 12.
+  static constexpr int SEG_COST = F32 || HD == 256 ? 4 : 8;
   static constexpr int VG = CB * 2048;       // 16 slots of a V piece: [block][16 slots][128 B]
 };
 // f32: tiles of a window.  Error against 64 bits of a 4100-token prompt and a 12000-token one: 3.1e-6 and 2.3e-6 with 4,
@@ -882,7 +883,8 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
             if (lane == 0) mbar_arrive(&c.full[slot]);
           }
         } else {
-          constexpr int KL = TC_KEYS / 32, VL = VK / 32, UR = HD / 8, VR = 32 / UR;  // rows a lane looks up; V: units of a row, rows a step
+          // rows a lane looks up (K, V); V: units of a row, rows a step
+          constexpr int KL = TC_KEYS / 32, VL = VK / 32, UR = HD / 8, VR = 32 / UR;
           const T *base = (const T *)(TREE ? (is_v ? a.kv.v : a.kv.k) : (is_v ? a.v : a.k));
           const int64_t rs = TREE ? (int64_t)a.nkv * HD : is_v ? a.vrow : a.krow, hs = TREE ? HD : is_v ? a.vhead : a.khead;
           base += g.hk * hs;
@@ -897,21 +899,22 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
             const int pick = is_v ? i8 * VR / 4 : i8;
             const int64_t mine_r = pick == 0 ? off[0] : pick == 1 ? off[1] : pick == 2 ? off[2] : off[3];
 #pragma unroll
-          for (int ii = 0; ii < 8; ii++) {
-            const int i = i8 * 8 + ii;
-            const int key = is_v ? i * VR + lane / UR : i * 4 + (lane >> 3), u = is_v ? lane % UR : b * 8 + (lane & 7);
-            const int64_t r = __shfl_sync(0xffffffffu, mine_r, key & 31);
-            const T *src = base + (r < 0 ? 0 : r * rs + u * 8);
-            uint8_t *d = dst + (((u & 7) ^ (key & 7)) << 4) + (is_v ? (key >> 4) * G_::VG + (u >> 3) * 2048 + (key & 15) * 128 : key * 128);
-            if (TREE || a.vec) {
-              cp_async16(smem_u32(d), src, r >= 0);
-            } else {
-              T e[8];
+            for (int ii = 0; ii < 8; ii++) {
+              const int i = i8 * 8 + ii;
+              const int key = is_v ? i * VR + lane / UR : i * 4 + (lane >> 3), u = is_v ? lane % UR : b * 8 + (lane & 7);
+              const int64_t r = __shfl_sync(0xffffffffu, mine_r, key & 31);
+              const T *src = base + (r < 0 ? 0 : r * rs + u * 8);
+              uint8_t *d = dst + (((u & 7) ^ (key & 7)) << 4) +
+                           (is_v ? (key >> 4) * G_::VG + (u >> 3) * 2048 + (key & 15) * 128 : key * 128);
+              if (TREE || a.vec) {
+                cp_async16(smem_u32(d), src, r >= 0);
+              } else {
+                T e[8];
 #pragma unroll
-              for (int k = 0; k < 8; k++) e[k] = r >= 0 ? src[k] : from_f<T>(0.f);
-              *(uint4 *)d = *(uint4 *)e;
+                for (int k = 0; k < 8; k++) e[k] = r >= 0 ? src[k] : from_f<T>(0.f);
+                *(uint4 *)d = *(uint4 *)e;
+              }
             }
-          }
           }
           cp_async_commit();
           cp_async_wait<0>();

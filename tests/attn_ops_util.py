@@ -78,7 +78,7 @@ class Cache:
 
     def rows(self, s, slots):
         """Flat pool rows of a sequence's slots."""
-        slots = torch.as_tensor(slots)
+        slots = torch.as_tensor(list(slots), dtype=torch.long)
         return (self.table_h[s].long()[slots // self.page] * self.page + slots % self.page).to(self.dev)
 
     def flat(self, which, layer=0):

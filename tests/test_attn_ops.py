@@ -404,6 +404,20 @@ def test_prompt_maximum_jumps(cw, t, hd):
     check_prompt(o[0], t, [n], 1, 1, q[0], k[0], v[0], 0.25)
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("odd", [False, True])
+def test_prompt_long(cw, t, hd, odd):
+    """Rows of many tiles (for f32 of several windows, added up in the output), also in rows that no vector access fits."""
+    g, lens, nh, nkv = gen(17), [2300, 1, 1153], 2, 1
+    n = sum(lens)
+    q, k, v, o = (rows_of(g, n, h, hd, t, None, hd + 3 if odd else None, 1 if odd else 0) for h in (nh, nkv, nkv, nh))
+    k[0][2000] *= 3.0  # the maximum of many rows comes late
+    o[0].fill_(math.nan)
+    run_prompt(cw, t, lens, nh, nkv, hd, None, q, k, v, o)
+    check_prompt(o[0], t, lens, nh, nkv, q[0], k[0], v[0], hd ** -0.5)
+
+
 @pytest.mark.parametrize("hd", [64, 256])
 @pytest.mark.parametrize("first,rest", [(0.0, 1e-4), (1.0, 1e6), (1e6, 1.0), (1e-20, 1e-20), (1e15, 1e15)])
 @pytest.mark.parametrize("what", ["k", "v"])
@@ -647,6 +661,55 @@ def test_tree_shared_pages_and_strided_rows(cw):
         masks = tree_masks(random.Random(1), 2, T)
         run_tree(cw, c, lens, T, nh, q, o, signed(masks))
         check_tree(c, o[0], q[0], lens, T, nh, masks, None, hd ** -0.5)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("n,T", [(40, 2), (130, 1), (300, 5)])
+def test_tree_many_sequences(cw, t, n, T):
+    """More sequences than a warp has lanes, some of them without nodes, lengths of none to a few tiles."""
+    g, rng, nh, nkv, hd = gen(n), random.Random(n), 4, 2, 64
+    lens = [rng.choice([0, 1, 5, 127, 128, 129, 400]) for _ in range(n)]
+    nodes = [rng.choice([0, 1, T, T]) for _ in range(n)]
+    c = Cache(cw, t, n, 400 + T, 16, nkv, hd)
+    fill(c, lens, nodes, g)
+    q, o = rows_of(g, n * T, nh, hd, t), rows_of(g, n * T, nh, hd, t)
+    o[0].fill_(3.0)
+    run_tree(cw, c, lens, T, nh, q, o, None, nodes)
+    check_tree(c, o[0], q[0], lens, T, nh, None, nodes, hd ** -0.5)
+    for s in range(n):
+        assert (o[0][s * T + nodes[s]:(s + 1) * T] == 3).all()
+    assert status(cw) == 0
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_cache_of_more_than_2_31_elements(cw, t):
+    """K and V pools of 2.1 G elements each: rows are written, read and moved on both sides of 2^31."""
+    g, T, nh, nkv, hd = gen(19), 4, 8, 8, 256
+    c = Cache(cw, t, 2, 700, 64, nkv, hd, spare=16500)
+    n = c.desc.n_pages
+    assert n * 64 * nkv * hd > 2 ** 31
+    half = c.stride // 2
+    c.table_h[0] = torch.arange(n - c.stride, n)  # the last pages, the first, and some of both
+    c.table_h[1] = torch.cat([torch.arange(half), torch.arange(n - 2 * c.stride, n - 2 * c.stride + c.stride - half)])
+    c.table.copy_(c.table_h)
+    lens = [600, 690]
+    rows = 600 + 690 + 2 * T
+    k, v = (normal(g, rows, nkv, hd, t=t) for _ in range(2))
+    seq = torch.tensor([0] * (600 + T) + [1] * (690 + T), device="cuda", dtype=torch.int32)
+    slot = torch.cat([torch.arange(600 + T), torch.arange(690 + T)]).int().cuda()
+    cw.check(cw.lib().cwen_cuda_kv_append(c.desc, 0, ptr(c.table), c.stride, 2, t, rows, ptr(k), nkv * hd, hd, ptr(v), nkv * hd,
+                                          hd, ptr(seq), ptr(slot), None, None, stream()))
+    at = torch.cat([c.rows(0, range(600 + T)), c.rows(1, range(690 + T))])
+    assert torch.equal(c.flat("k")[at], k) and torch.equal(c.flat("v")[at], v)
+    q, o = rows_of(g, 2 * T, nh, hd, t), rows_of(g, 2 * T, nh, hd, t)
+    run_tree(cw, c, lens, T, nh, q, o)
+    check_tree(c, o[0], q[0], lens, T, nh, None, None, hd ** -0.5)
+    ln, kp = torch.tensor(lens, device="cuda", dtype=torch.int32), torch.tensor([0b1010, 0b1000], device="cuda")
+    cw.check(cw.lib().cwen_cuda_kv_compact(c.desc, ptr(c.table), c.stride, 2, ptr(ln), ptr(kp), None, stream()))
+    now = torch.cat([c.rows(0, [600, 601]), c.rows(1, [690])])
+    assert torch.equal(c.flat("k")[now], k[[601, 603, 600 + T + 693]])
+    assert torch.equal(c.flat("v")[now], v[[601, 603, 600 + T + 693]])
+    assert status(cw) == 0
 
 
 # ------------------------------------------------------------------ streams and graphs

@@ -1075,6 +1075,18 @@ __global__ void __launch_bounds__(Geo<TY, HD>::THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 8; k++) x[i][k] = src[i][k];
         }
+        if constexpr (TREE) {
+          // one piece in registers does not cover the memory's latency: a 128-byte line a thread, of the tile that
+          // comes next in K or in V, into the L2 (8 ragged sequences of 8 kv heads of 128, one token each 217 -> 198 us,
+          // trees of 24 nodes 234 -> 227 us; the chain of 9 over 4 heads of 256 as before)
+          if (tile + 1 < g.w1) {
+            const uint32_t o = rowoff[(tile + 1) & 3][lt >> 1];
+            if (o != NONE) {
+              const float *line = (const float *)(is_v ? a.kv.v : a.kv.k) + ((int64_t)o * a.nkv + g.hk) * HD + (2 * pb + (lt & 1)) * 32;
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            }
+          }
+        }
       };
       float fk = 1.f, fv = 1.f;
       bool have = advance();
